@@ -193,6 +193,102 @@ int sg_expand_chain(const int32_t* cont, int32_t rows, int32_t max_occ,
                     int64_t* num_valid, int64_t* num_emit, float* score,
                     sg_stream_t stream);
 
+/* ---- draft verification (no reference counterpart: the reference stops at
+ * the drafts and takes the sampled ids back; these calls turn the target
+ * model's logits and the drafts into those ids and counts) ---------------
+ *
+ * One row l of logits (NaN read as -inf; m its largest value) under a
+ * temperature T, top-k and top-p gives the target's probabilities P:
+ *   w_i = exp((l_i - m) / T); -inf has weight 0, and where m = +inf the
+ *   +inf entries share the mass;
+ *   top-k (0 < k < V) keeps the values >= the k-th largest (all of a tie);
+ *   top-p (p < 1) keeps, of those, the values >= t, t the largest value
+ *   whose tokens >= t hold at least p of the kept mass (p <= 0: the largest
+ *   value only), so tokens of one value stay or go together;
+ *   P_i = w_i / the sum of the kept weights.
+ *   T not > 0: P is 1 at the first largest token. A row whose entries are
+ *   all -inf has no mass: P = 0.
+ * Draft j (j < n = min(num_valid, K)) with token x is accepted while
+ * 0 <= x < V and u_j * q_j(x) < P_j(x) (q = 1 where drafts come without
+ * probabilities). At the first rejection s (s = n when there is none) one
+ * more token is drawn: the lowest i whose running sum of r exceeds u_K
+ * times the sum of r, where r = P_s with the rejected token left out
+ * (max(P_s - q_s, 0) with draft probabilities), or P_s itself when s = n
+ * or nothing is left. The request's output is its accepted drafts, that
+ * token and -1 from there on; count is the number of tokens. A row without
+ * mass gives no token. num_valid < 0 marks an inactive request: all -1,
+ * count 0, none of its rows read. Every decision is the one 64-bit
+ * arithmetic on the inputs gives. */
+#define SG_F32 0
+#define SG_BF16 1
+#define SG_F16 2
+
+/* Rows of logits or probabilities, a row for each request and position.
+ * row_start NULL: row j of request b starts at element
+ * b * stride_b + j * stride_j. Otherwise rows are packed, stride_b elements
+ * apart, and row j of request b is row row_start[b] + j of n_rows; a row
+ * outside [0, n_rows) counts as one without mass. */
+typedef struct sg_rows {
+  const void* data;
+  int32_t dtype;     /* SG_F32, SG_BF16, SG_F16 */
+  int32_t batch;     /* B: requests */
+  int32_t positions; /* rows of a request: K + 1 for K drafts */
+  int32_t pad_;
+  int64_t vocab;     /* V: elements of a row (unit stride) */
+  int64_t stride_b;
+  int64_t stride_j;
+  const int32_t* row_start; /* [B] or NULL */
+  int64_t n_rows;
+} sg_rows;
+
+/* Sampling settings, per request ([B] device arrays) or, where the pointer
+ * is NULL, one value for all. */
+typedef struct sg_sampling {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  float temperature_all;
+  int32_t top_k_all; /* <= 0: off */
+  float top_p_all;   /* >= 1: off */
+  int32_t pad_;
+} sg_sampling;
+
+/* Workspace bytes of sg_verify_greedy, sg_verify_sampled and
+ * sg_target_probs. Calls that may overlap on the GPU (other streams, other
+ * graphs) need workspaces of their own. */
+size_t sg_verify_workspace_size(int32_t batch, int32_t positions);
+
+/* Verification at temperature 0: each accepted draft equals its row's first
+ * largest token. draft is [B, K] int32 with K = positions - 1, num_valid
+ * [B] or NULL (all K), sampled [B, K + 1] int32, count [B] int32. */
+int sg_verify_greedy(const sg_rows* logits, const int32_t* draft,
+                     const int32_t* num_valid, int32_t* sampled,
+                     int32_t* count, void* workspace, size_t workspace_bytes,
+                     sg_stream_t stream);
+
+/* Verification by given random numbers, from logits; the probabilities are
+ * not stored. uniforms is [B, K + 1] fp32 in [0, 1): columns 0..K-1 accept
+ * the drafts, column K draws the token after them. */
+int sg_verify_sampled(const sg_rows* logits, const sg_sampling* sampling,
+                      const int32_t* draft, const int32_t* num_valid,
+                      const float* uniforms, int32_t* sampled, int32_t* count,
+                      void* workspace, size_t workspace_bytes,
+                      sg_stream_t stream);
+
+/* Verification from probabilities (fp32 rows; values that are negative or
+ * not finite count as 0) against one-hot drafts (draft_probs NULL) or the
+ * drafter's own distribution (fp32 rows, positions = K). */
+int sg_verify_probs(const sg_rows* probs, const sg_rows* draft_probs,
+                    const int32_t* draft, const int32_t* num_valid,
+                    const float* uniforms, int32_t* sampled, int32_t* count,
+                    sg_stream_t stream);
+
+/* The target's probabilities P of every row, out [B, positions, V] fp32
+ * (contiguous). */
+int sg_target_probs(const sg_rows* logits, const sg_sampling* sampling,
+                    float* out, void* workspace, size_t workspace_bytes,
+                    sg_stream_t stream);
+
 /* ---- vLLM glue ----------------------------------------------------------- */
 
 /* The per-step preparation of vLLM's GPU n-gram proposer

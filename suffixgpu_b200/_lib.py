@@ -62,6 +62,33 @@ class LocalOutputs(Structure):
     ]
 
 
+class Rows(Structure):
+    _fields_ = [
+        ("data", c_void_p),
+        ("dtype", c_int32),
+        ("batch", c_int32),
+        ("positions", c_int32),
+        ("pad_", c_int32),
+        ("vocab", c_int64),
+        ("stride_b", c_int64),
+        ("stride_j", c_int64),
+        ("row_start", c_void_p),
+        ("n_rows", c_int64),
+    ]
+
+
+class Sampling(Structure):
+    _fields_ = [
+        ("temperature", c_void_p),
+        ("top_k", c_void_p),
+        ("top_p", c_void_p),
+        ("temperature_all", c_float),
+        ("top_k_all", c_int32),
+        ("top_p_all", c_float),
+        ("pad_", c_int32),
+    ]
+
+
 # name -> (argtypes); every entry point returns int status
 _SIGS: dict[str, list] = {
     "sg_local_draft": [POINTER(DraftParams), POINTER(LocalInputs),
@@ -130,6 +157,15 @@ _SIGS: dict[str, list] = {
                                 c_int32, c_float, c_float, c_float, c_float,
                                 c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_void_p],
+    "sg_verify_greedy": [POINTER(Rows), c_void_p, c_void_p, c_void_p,
+                         c_void_p, c_void_p, c_size_t, c_void_p],
+    "sg_verify_sampled": [POINTER(Rows), POINTER(Sampling), c_void_p,
+                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                          c_size_t, c_void_p],
+    "sg_verify_probs": [POINTER(Rows), POINTER(Rows), c_void_p, c_void_p,
+                        c_void_p, c_void_p, c_void_p, c_void_p],
+    "sg_target_probs": [POINTER(Rows), POINTER(Sampling), c_void_p, c_void_p,
+                        c_size_t, c_void_p],
     "sg_global_combine": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                           c_void_p, c_void_p, c_int32, c_int32, c_int32,
                           c_void_p],
@@ -172,6 +208,7 @@ _SIGS_EXTRA: dict[str, tuple] = {
     "sg_set_wait_polls": (c_int, [c_int]),
     "sg_suffix_array_append_workspace_size": (c_size_t, [c_int64]),
     "sg_shard_extract_workspace_size": (c_size_t, [c_int64]),
+    "sg_verify_workspace_size": (c_size_t, [c_int32, c_int32]),
 }
 
 
@@ -238,5 +275,6 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-__all__ = ["DraftParams", "LocalInputs", "LocalOutputs", "lib", "call",
-           "check", "ptr", "stream_of", "register", "c_size_t"]
+__all__ = ["DraftParams", "LocalInputs", "LocalOutputs", "Rows", "Sampling",
+           "lib", "call", "check", "ptr", "stream_of", "register",
+           "c_size_t"]

@@ -14,6 +14,9 @@
 // taken to be written by the CPU (not by GPU work still in flight).
 // suffixgpu_b200::vllm_prepare wraps sg_vllm_prepare, the per-step input
 // preparation of vLLM's GPU n-gram proposer, for the vLLM adapter.
+// suffixgpu_b200::verify_greedy / verify_sampled / verify_probs /
+// target_probs wrap the draft-verification entry points; their argument
+// checks run before any CUDA call (and raise ValueError).
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -21,8 +24,10 @@
 
 #include <cuda_runtime_api.h>
 
+#include <algorithm>
 #include <cstring>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "../../include/suffixgpu.h"
@@ -349,6 +354,269 @@ int64_t global_finish(at::TensorList found, const at::Tensor& row_mask,
   return SG_OK;
 }
 
+// ---- draft verification (sg_verify_greedy / _sampled / _probs,
+// sg_target_probs). Arguments are checked before anything touches the GPU.
+
+// Rows of logits or probabilities: [B, positions, V] or, with row_start,
+// packed [N, V].
+sg_rows rows_of(const at::Tensor& t, const char* what, int64_t b,
+                int64_t positions, const c10::optional<at::Tensor>& row_start) {
+  const std::string name(what);
+  sg_rows r{};
+  switch (t.scalar_type()) {
+    case at::kFloat: r.dtype = SG_F32; break;
+    case at::kBFloat16: r.dtype = SG_BF16; break;
+    case at::kHalf: r.dtype = SG_F16; break;
+    default:
+      TORCH_CHECK_VALUE(false, name +
+                        " must be a float32, bfloat16 or float16 tensor");
+  }
+  if (row_start.has_value()) {
+    TORCH_CHECK_VALUE(t.dim() == 2, name +
+                      " must be [N, V] when row_start is given");
+    TORCH_CHECK_VALUE(row_start->dim() == 1 && row_start->size(0) == b,
+                      "row_start must be a [B] tensor");
+    r.n_rows = t.size(0);
+  } else {
+    TORCH_CHECK_VALUE(t.dim() == 3, name +
+                      " must be [B, K + 1, V], or [N, V] with row_start");
+    TORCH_CHECK_VALUE(t.size(0) == b && t.size(1) >= positions,
+                      name + " must hold a row for every position of every "
+                      "request");
+    r.stride_j = t.stride(1);
+  }
+  r.stride_b = t.stride(0);
+  r.vocab = t.size(-1);
+  TORCH_CHECK_VALUE(r.vocab >= 1, name + " has an empty vocabulary");
+  TORCH_CHECK_VALUE(t.stride(-1) == 1 || r.vocab == 1,
+                    name + " must have unit stride over the vocabulary");
+  TORCH_CHECK_VALUE(b <= INT32_MAX && positions <= INT32_MAX,
+                    "too many requests or positions");
+  r.batch = static_cast<int32_t>(b);
+  r.positions = static_cast<int32_t>(positions);
+  return r;
+}
+
+// An index tensor as contiguous int32 on `dev`.
+at::Tensor index_i32(const at::Tensor& t, const char* what,
+                     const at::Device& dev) {
+  const at::ScalarType s = t.scalar_type();
+  TORCH_CHECK_VALUE(s == at::kInt || s == at::kLong || s == at::kShort,
+                    std::string(what) + " must be an integer tensor");
+  TORCH_CHECK_VALUE(t.device() == dev,
+                    std::string(what) + " is on another device");
+  return s == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+}
+
+// The per-request setting tensors as the struct the kernels take; `keep`
+// holds the converted tensors until the launch.
+sg_sampling sampling_of(const c10::optional<at::Tensor>& temperature,
+                        const c10::optional<at::Tensor>& top_k,
+                        const c10::optional<at::Tensor>& top_p,
+                        double temperature_all, int64_t top_k_all,
+                        double top_p_all, int64_t b, const at::Device& dev,
+                        std::vector<at::Tensor>* keep) {
+  sg_sampling s{};
+  s.temperature_all = static_cast<float>(temperature_all);
+  s.top_k_all = static_cast<int32_t>(
+      std::max<int64_t>(0, std::min<int64_t>(top_k_all, INT32_MAX)));
+  s.top_p_all = static_cast<float>(top_p_all);
+  auto check = [&](const at::Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == b, std::string(what) +
+                      " must be a number or a [B] tensor");
+    TORCH_CHECK_VALUE(t.device() == dev,
+                      std::string(what) + " is on another device");
+  };
+  auto real = [&](const at::Tensor& t, const char* what) {
+    check(t, what);
+    TORCH_CHECK_VALUE(at::isFloatingType(t.scalar_type()),
+                      std::string(what) + " must be a floating tensor");
+    keep->push_back(t.to(at::kFloat).contiguous());
+    return keep->back().data_ptr<float>();
+  };
+  if (temperature.has_value()) s.temperature = real(*temperature, "temperature");
+  if (top_p.has_value()) s.top_p = real(*top_p, "top_p");
+  if (top_k.has_value()) {
+    check(*top_k, "top_k");
+    keep->push_back(index_i32(*top_k, "top_k", dev));
+    s.top_k = keep->back().data_ptr<int32_t>();
+  }
+  return s;
+}
+
+// What the three verify operators share: the checked index tensors, the
+// output buffer and the launch stream.
+struct VerifyCall {
+  int64_t b = 0, k = 0;
+  at::Tensor draft, num_valid, row_start, uniforms, buf;
+  const int32_t* draft_ptr = nullptr;
+  const int32_t* nv_ptr = nullptr;
+  int32_t* sampled = nullptr;
+  int32_t* count = nullptr;
+
+  VerifyCall(const at::Tensor& rows, const at::Tensor& draft_in,
+             const c10::optional<at::Tensor>& num_valid_in,
+             const c10::optional<at::Tensor>& row_start_in,
+             const c10::optional<at::Tensor>& uniforms_in) {
+    const at::Device dev = rows.device();
+    TORCH_CHECK_VALUE(draft_in.dim() == 2, "draft must be a [B, K] tensor");
+    b = draft_in.size(0);
+    k = draft_in.size(1);
+    draft = index_i32(draft_in, "draft", dev);
+    if (num_valid_in.has_value()) {
+      TORCH_CHECK_VALUE(num_valid_in->dim() == 1 && num_valid_in->size(0) == b,
+                        "num_valid must be a [B] tensor");
+      num_valid = index_i32(*num_valid_in, "num_valid", dev);
+    }
+    if (row_start_in.has_value())
+      row_start = index_i32(*row_start_in, "row_start", dev);
+    if (uniforms_in.has_value()) {
+      TORCH_CHECK_VALUE(uniforms_in->scalar_type() == at::kFloat &&
+                            uniforms_in->dim() == 2 &&
+                            uniforms_in->size(0) == b &&
+                            uniforms_in->size(1) == k + 1,
+                        "uniforms must be a float32 [B, K + 1] tensor");
+      TORCH_CHECK_VALUE(uniforms_in->device() == dev,
+                        "uniforms is on another device");
+      uniforms = uniforms_in->contiguous();
+    }
+  }
+
+  // Pointers, once every check has passed and the tensors are on a GPU.
+  void begin(const at::Tensor& rows, sg_rows* r) {
+    TORCH_CHECK_VALUE(rows.is_cuda(),
+                      "suffixgpu_b200 ops need CUDA tensors");
+    r->data = rows.data_ptr();
+    if (row_start.defined()) r->row_start = row_start.data_ptr<int32_t>();
+    buf = at::empty({b * (k + 2)}, draft.options());
+    sampled = buf.data_ptr<int32_t>();
+    count = sampled + b * (k + 1);
+    draft_ptr = draft.data_ptr<int32_t>();
+    if (num_valid.defined()) nv_ptr = num_valid.data_ptr<int32_t>();
+  }
+
+  std::tuple<at::Tensor, at::Tensor> result() const {
+    return {buf.narrow(0, 0, b * (k + 1)).view({b, k + 1}),
+            buf.narrow(0, b * (k + 1), b)};
+  }
+};
+
+sg_stream_t stream_for(const at::Tensor& t) {
+  return reinterpret_cast<sg_stream_t>(
+      c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
+}
+
+// A workspace of the call's own: calls on other streams and other captured
+// graphs never share one.
+at::Tensor verify_workspace(const sg_rows& r, const at::Tensor& like) {
+  return at::empty({static_cast<int64_t>(
+                       sg_verify_workspace_size(r.batch, r.positions)) + 16},
+                   like.options().dtype(at::kByte));
+}
+
+std::tuple<at::Tensor, at::Tensor> verify_greedy(
+    const at::Tensor& logits, const at::Tensor& draft,
+    const c10::optional<at::Tensor>& num_valid,
+    const c10::optional<at::Tensor>& row_start) {
+  VerifyCall c(logits, draft, num_valid, row_start, c10::nullopt);
+  sg_rows r = rows_of(logits, "logits", c.b, c.k + 1, row_start);
+  TORCH_CHECK_VALUE(logits.is_cuda(), "suffixgpu_b200 ops need CUDA tensors");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  c.begin(logits, &r);
+  at::Tensor ws = verify_workspace(r, logits);
+  check_status("sg_verify_greedy",
+               sg_verify_greedy(&r, c.draft_ptr, c.nv_ptr, c.sampled, c.count,
+                                ws.data_ptr(), ws.numel(),
+                                stream_for(logits)));
+  return c.result();
+}
+
+std::tuple<at::Tensor, at::Tensor> verify_sampled(
+    const at::Tensor& logits, const at::Tensor& draft,
+    const at::Tensor& uniforms, const c10::optional<at::Tensor>& num_valid,
+    const c10::optional<at::Tensor>& temperature,
+    const c10::optional<at::Tensor>& top_k,
+    const c10::optional<at::Tensor>& top_p, double temperature_all,
+    int64_t top_k_all, double top_p_all,
+    const c10::optional<at::Tensor>& row_start) {
+  VerifyCall c(logits, draft, num_valid, row_start, uniforms);
+  sg_rows r = rows_of(logits, "logits", c.b, c.k + 1, row_start);
+  std::vector<at::Tensor> keep;
+  sg_sampling s = sampling_of(temperature, top_k, top_p, temperature_all,
+                              top_k_all, top_p_all, c.b, logits.device(),
+                              &keep);
+  TORCH_CHECK_VALUE(logits.is_cuda(), "suffixgpu_b200 ops need CUDA tensors");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  c.begin(logits, &r);
+  at::Tensor ws = verify_workspace(r, logits);
+  check_status("sg_verify_sampled",
+               sg_verify_sampled(&r, &s, c.draft_ptr, c.nv_ptr,
+                                 c.uniforms.data_ptr<float>(), c.sampled,
+                                 c.count, ws.data_ptr(), ws.numel(),
+                                 stream_for(logits)));
+  return c.result();
+}
+
+std::tuple<at::Tensor, at::Tensor> verify_probs(
+    const at::Tensor& probs, const at::Tensor& draft,
+    const at::Tensor& uniforms, const c10::optional<at::Tensor>& num_valid,
+    const c10::optional<at::Tensor>& draft_probs,
+    const c10::optional<at::Tensor>& row_start) {
+  TORCH_CHECK_VALUE(probs.scalar_type() == at::kFloat,
+                    "probs must be a float32 tensor");
+  VerifyCall c(probs, draft, num_valid, row_start, uniforms);
+  sg_rows r = rows_of(probs, "probs", c.b, c.k + 1, row_start);
+  sg_rows q{};
+  if (draft_probs.has_value()) {
+    TORCH_CHECK_VALUE(draft_probs->scalar_type() == at::kFloat,
+                      "draft_probs must be a float32 tensor");
+    q = rows_of(*draft_probs, "draft_probs", c.b, c.k, c10::nullopt);
+    TORCH_CHECK_VALUE(q.vocab == r.vocab,
+                      "draft_probs and probs differ in vocabulary");
+    TORCH_CHECK_VALUE(draft_probs->device() == probs.device(),
+                      "draft_probs is on another device");
+  }
+  TORCH_CHECK_VALUE(probs.is_cuda(), "suffixgpu_b200 ops need CUDA tensors");
+  const c10::cuda::CUDAGuard guard(probs.device());
+  c.begin(probs, &r);
+  if (draft_probs.has_value()) q.data = draft_probs->data_ptr();
+  check_status("sg_verify_probs",
+               sg_verify_probs(&r, draft_probs.has_value() ? &q : nullptr,
+                               c.draft_ptr, c.nv_ptr,
+                               c.uniforms.data_ptr<float>(), c.sampled,
+                               c.count, stream_for(probs)));
+  return c.result();
+}
+
+at::Tensor target_probs(const at::Tensor& logits,
+                        const c10::optional<at::Tensor>& temperature,
+                        const c10::optional<at::Tensor>& top_k,
+                        const c10::optional<at::Tensor>& top_p,
+                        double temperature_all, int64_t top_k_all,
+                        double top_p_all) {
+  TORCH_CHECK_VALUE(logits.dim() == 2 || logits.dim() == 3,
+                    "logits must be [N, V] or [B, J, V]");
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && logits.requires_grad()),
+                    "target_probs has no backward pass: detach the logits "
+                    "or call it under torch.no_grad()");
+  const at::Tensor rows = logits.dim() == 3 ? logits : logits.unsqueeze(1);
+  sg_rows r = rows_of(rows, "logits", rows.size(0), rows.size(1),
+                      c10::nullopt);
+  std::vector<at::Tensor> keep;
+  sg_sampling s = sampling_of(temperature, top_k, top_p, temperature_all,
+                              top_k_all, top_p_all, r.batch, rows.device(),
+                              &keep);
+  TORCH_CHECK_VALUE(rows.is_cuda(), "suffixgpu_b200 ops need CUDA tensors");
+  const c10::cuda::CUDAGuard guard(rows.device());
+  r.data = rows.data_ptr();
+  at::Tensor out = at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
+  at::Tensor ws = verify_workspace(r, rows);
+  check_status("sg_target_probs",
+               sg_target_probs(&r, &s, out.data_ptr<float>(), ws.data_ptr(),
+                               ws.numel(), stream_for(rows)));
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(suffixgpu_b200, m) {
@@ -374,6 +642,31 @@ TORCH_LIBRARY(suffixgpu_b200, m) {
       "float spec_factor, float spec_offset, float min_prob, float alpha, "
       "Tensor local_score, Tensor draft, Tensor num_valid, int s0, int s1, "
       "int ev2, int ev3) -> int");
+  m.def(
+      "verify_greedy(Tensor logits, Tensor draft, Tensor? num_valid, "
+      "Tensor? row_start) -> (Tensor, Tensor)");
+  m.def(
+      "verify_sampled(Tensor logits, Tensor draft, Tensor uniforms, "
+      "Tensor? num_valid, Tensor? temperature, Tensor? top_k, "
+      "Tensor? top_p, float temperature_all, int top_k_all, "
+      "float top_p_all, Tensor? row_start) -> (Tensor, Tensor)");
+  m.def(
+      "verify_probs(Tensor probs, Tensor draft, Tensor uniforms, "
+      "Tensor? num_valid, Tensor? draft_probs, Tensor? row_start) "
+      "-> (Tensor, Tensor)");
+  m.def(
+      "target_probs(Tensor logits, Tensor? temperature, Tensor? top_k, "
+      "Tensor? top_p, float temperature_all, int top_k_all, "
+      "float top_p_all) -> Tensor");
+}
+
+// The verification operators check their arguments (tensors' devices among
+// them) themselves, so one registration covers every device.
+TORCH_LIBRARY_IMPL(suffixgpu_b200, CompositeExplicitAutograd, m) {
+  m.impl("verify_greedy", &verify_greedy);
+  m.impl("verify_sampled", &verify_sampled);
+  m.impl("verify_probs", &verify_probs);
+  m.impl("target_probs", &target_probs);
 }
 
 TORCH_LIBRARY_IMPL(suffixgpu_b200, CUDA, m) {

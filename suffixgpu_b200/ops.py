@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from suffixgpu_b200 import _lib
-from suffixgpu_b200._lib import call, ptr, stream_of
+from suffixgpu_b200._lib import call, ptr, stream_of, torch_ops
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
@@ -245,3 +245,97 @@ def longest_suffix_match(sa, corpus, query, query_len, max_len: int):
     best, s, e = suffix_match_backoff(sa, corpus, query, query_len, max_len,
                                       caps)
     return best[:, 0], s[:, 0], e[:, 0]
+
+
+# ---------------------------------------------------------------------------
+# draft verification (no reference counterpart: the reference ends at the
+# drafts and takes the sampled ids back)
+# ---------------------------------------------------------------------------
+def _setting(value, off):
+    """(tensor, number) of a per-request setting: one of the two is used."""
+    if value is None:
+        return None, off
+    if isinstance(value, torch.Tensor):
+        return value, off
+    return None, value
+
+
+def verify_greedy(logits: torch.Tensor, draft: torch.Tensor,
+                  num_valid: torch.Tensor | None = None,
+                  row_start: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Verification of drafts at temperature 0: each request's drafts are
+    accepted while they equal the first largest token of their logits row,
+    and the row after them gives one more token.
+
+    logits: float32, bfloat16 or float16, [B, K + 1, V] (row j is the
+    target's after draft j - 1; any strides over the first two dimensions),
+    or packed [N, V] with row_start [B], request b's rows starting at
+    row_start[b]. draft: [B, K] token ids. num_valid [B]: drafts of each
+    request that count (None: K; negative: an inactive request, whose rows
+    are not read). NaN logits count as masked (-inf).
+
+    Returns (sampled [B, K + 1] int32, -1 past the count; count [B] int32),
+    what propose_with_update takes as its sampled ids and their count. A
+    row with nothing but -inf ends its request without a token."""
+    return torch_ops().verify_greedy(logits, draft, num_valid, row_start)
+
+
+def verify_sampled(logits: torch.Tensor, draft: torch.Tensor,
+                   uniforms: torch.Tensor,
+                   num_valid: torch.Tensor | None = None,
+                   temperature: torch.Tensor | float = 1.0,
+                   top_k: torch.Tensor | int | None = None,
+                   top_p: torch.Tensor | float | None = None,
+                   row_start: torch.Tensor | None = None
+                   ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Verification of drafts that keeps the target's distribution, from its
+    logits and given random numbers; probabilities are not stored.
+
+    Draft j (token x) is accepted while uniforms[b, j] < P_j(x); at the
+    first rejection, or after the last draft, one more token is drawn with
+    uniforms[b, K] by inverse CDF over token ids, from the row's P without
+    the rejected token. uniforms: [B, K + 1] float32 in [0, 1).
+
+    temperature, top_k, top_p: numbers or [B] tensors, floats rounded to
+    float32. P is softmax(l / T) over the tokens that top_k (values >= the
+    k-th largest, ties kept; 0 = off) and then top_p (the values >= t, t the
+    largest one whose tokens >= t hold at least top_p of the kept mass;
+    1 = off) leave. T <= 0 is greedy. Other arguments and the result as
+    verify_greedy's. Decisions are those of 64-bit arithmetic on the logits
+    as stored."""
+    t, t_all = _setting(temperature, 1.0)
+    k, k_all = _setting(top_k, 0)
+    p, p_all = _setting(top_p, 1.0)
+    return torch_ops().verify_sampled(logits, draft, uniforms, num_valid, t,
+                                      k, p, t_all, k_all, p_all, row_start)
+
+
+def verify_probs(probs: torch.Tensor, draft: torch.Tensor,
+                 uniforms: torch.Tensor,
+                 num_valid: torch.Tensor | None = None,
+                 draft_probs: torch.Tensor | None = None,
+                 row_start: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+    """verify_sampled from float32 probabilities ([B, K + 1, V], or packed
+    [N, V] with row_start). With draft_probs [B, K, V] float32, the
+    distributions the drafts were drawn from, draft j is accepted while
+    uniforms[b, j] * q_j(x) < p_j(x), and the token after a rejection is
+    drawn from max(p - q, 0). Values that are negative or not finite count
+    as 0; a row without mass ends its request without a token."""
+    return torch_ops().verify_probs(probs, draft, uniforms, num_valid,
+                                    draft_probs, row_start)
+
+
+def target_probs(logits: torch.Tensor,
+                 temperature: torch.Tensor | float = 1.0,
+                 top_k: torch.Tensor | int | None = None,
+                 top_p: torch.Tensor | float | None = None) -> torch.Tensor:
+    """The target's probabilities under verify_sampled's temperature, top_k
+    and top_p, float32 in the shape of logits ([N, V] with [N] settings, or
+    [B, J, V] with [B] settings; float32, bfloat16 or float16). Dropped
+    tokens are exactly 0; a row of -inf gives zeros. No backward pass."""
+    t, t_all = _setting(temperature, 1.0)
+    k, k_all = _setting(top_k, 0)
+    p, p_all = _setting(top_p, 1.0)
+    return torch_ops().target_probs(logits, t, k, p, t_all, k_all, p_all)

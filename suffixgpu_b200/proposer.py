@@ -199,6 +199,55 @@ class SuffixGPUDrafter:
         return self._into(out, *self.global_index.finish_global_step(
             pend, o, self, streams))
 
+    # ------------------------------------------------------------------
+    # verification (no reference counterpart: it ends at the drafts)
+    # ------------------------------------------------------------------
+    def verify(self, logits: torch.Tensor, draft: torch.Tensor,
+               num_valid: torch.Tensor | None = None,
+               uniforms: torch.Tensor | None = None,
+               temperature: torch.Tensor | float | None = None,
+               top_k: torch.Tensor | int | None = None,
+               top_p: torch.Tensor | float | None = None,
+               row_start: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+        """The target model's answer to this drafter's drafts: (sampled
+        [B, k+1] int32, count [B] int32), propose_with_update's next
+        ``sampled_token_ids`` and ``valid_sampled_tokens_count``. Without
+        ``uniforms`` the verification is greedy (ops.verify_greedy) and
+        takes no sampling settings; with them it keeps the target's
+        distribution (ops.verify_sampled). No host sync."""
+        if uniforms is None:
+            if not (temperature is None and top_k is None and top_p is None):
+                raise ValueError("temperature, top_k and top_p need uniforms "
+                                 "(without them verification is greedy)")
+            return ops.verify_greedy(logits, draft, num_valid, row_start)
+        return ops.verify_sampled(
+            logits, draft, uniforms, num_valid,
+            1.0 if temperature is None else temperature, top_k, top_p,
+            row_start)
+
+    def verify_and_propose(
+        self, logits: torch.Tensor, draft: torch.Tensor,
+        num_valid: torch.Tensor | None, num_tokens_no_spec: torch.Tensor,
+        token_ids_gpu: torch.Tensor,
+        uniforms: torch.Tensor | None = None,
+        temperature: torch.Tensor | float | None = None,
+        top_k: torch.Tensor | int | None = None,
+        top_p: torch.Tensor | float | None = None,
+        row_start: torch.Tensor | None = None,
+        max_model_len: int | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+               torch.Tensor]:
+        """One decode step after the target's forward pass: ``verify`` the
+        last drafts, then ``propose_with_update`` with what it sampled.
+        Returns (draft, num_valid, new_num_tokens, sampled, count). No host
+        sync; can be captured into a CUDA graph."""
+        sampled, count = self.verify(logits, draft, num_valid, uniforms,
+                                     temperature, top_k, top_p, row_start)
+        draft, num_valid, n = self.propose_with_update(
+            num_tokens_no_spec, token_ids_gpu, sampled, count, max_model_len)
+        return draft, num_valid, n, sampled, count
+
     def _on_device(self, t: torch.Tensor | None) -> torch.Tensor | None:
         if t is None or t.is_cuda:
             return t
