@@ -3,6 +3,7 @@
 // values are read and ordered, and a token's weight under a temperature.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -60,6 +61,47 @@ __device__ __forceinline__ double weight64(float l, float m, double inv_t) {
   if (l == m) return 1.0;
   if (l == -CUDART_INF_F || m == CUDART_INF_F) return 0.0;
   return exp((static_cast<double>(l) - static_cast<double>(m)) * inv_t);
+}
+
+// Exact weights: exp((l - m) / T) in 64 bits without branches, so that the
+// eight of a vector overlap (with a called exp() and its branches a block's
+// warps took 300 clocks each for a weight a lane). 2^y = 2^n * 2^(i / 16) *
+// 2^f with y = n + i / 16 + f, |f| <= 1 / 32: 2^(i / 16) from a table in
+// shared memory (16 doubles lie in the 32 banks without conflicts), 2^f by
+// its Taylor series to f^6 (the next term is below 2^-50). Weights below
+// 2^-1022 count as 0, and so do NaN and -inf. m is not +inf.
+constexpr int kExpTable = 16;
+
+__device__ __forceinline__ void fill_exp_table(double* tab) {
+  if (threadIdx.x < kExpTable) tab[threadIdx.x] = exp2(threadIdx.x / 16.0);
+}
+
+__device__ __forceinline__ double scale64_of(float t) {
+  return 1.4426950408889634074 / static_cast<double>(t);
+}
+
+__device__ __forceinline__ double weight64(float l, double m, double scale,
+                                           const double* tab) {
+  constexpr double c1 = 0.69314718055994530942;  // ln2^k / k!
+  constexpr double c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
+                   c5 = c4 * c1 / 5, c6 = c5 * c1 / 6;
+  const double y = (static_cast<double>(l) - m) * scale;
+  // 1.5 * 2^48: its unit is 1 / 16, so the sum's low word is 16 * y rounded
+  const double magic = 422212465065984.0;
+  const double t = y + magic;
+  const int i = __double2loint(t);
+  const double f = y - (t - magic);
+  double r = fma(f, c6, c5);
+  r = fma(f, r, c4);
+  r = fma(f, r, c3);
+  r = fma(f, r, c2);
+  r = fma(f, r, c1);
+  r = fma(f, r, 1.0);
+  r *= tab[i & (kExpTable - 1)];
+  r = __hiloint2double(__double2hiint(r) + ((i >> 4) << 20),
+                       __double2loint(r));
+  // y below -1022, infinite or NaN (-inf under an infinite temperature)
+  return (__double2hiint(y) & 0x7fffffff) > 0x408ff000 ? 0.0 : r;
 }
 
 // Probabilities read from memory: NaN, infinities and negative values
@@ -123,6 +165,345 @@ inline int check_rows(const sg_rows* r, bool probs) {
   }
   if (!r->data || r->stride_b < 0 || r->stride_j < 0) return SG_ERR_INVALID;
   return SG_OK;
+}
+
+// ---------------------------------------------------------------------------
+// A row as 16-byte vectors
+// ---------------------------------------------------------------------------
+// Rows start anywhere (odd vocabularies, slices), so a row is read on the
+// 16-byte grid of its addresses: vector v holds elements v * E - head + e,
+// e < E; the first and the last may stick out of the row, and are then read
+// element by element. Elements outside the row read as -inf.
+template <class T>
+struct RowVecs {
+  static constexpr int E = 16 / sizeof(T);
+  const T* row;
+  int64_t v;     // elements
+  int head;      // elements of the first vector that lie before the row
+  int nv;        // vectors
+  int in0, in1;  // vectors [in0, in1) lie wholly inside
+
+  __device__ __forceinline__ RowVecs(const T* r, int64_t vocab) : row(r) {
+    v = r ? vocab : 0;
+    head = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+    nv = v ? static_cast<int>((head + v + E - 1) / E) : 0;
+    in0 = head ? 1 : 0;
+    in1 = static_cast<int>((head + v) / E);
+  }
+  // Row index of a vector's first element.
+  __device__ __forceinline__ int64_t first(int vec) const {
+    return static_cast<int64_t>(vec) * E - head;
+  }
+  __device__ __forceinline__ bool inner(int vec) const {
+    return vec >= in0 && vec < in1;
+  }
+};
+
+template <class T>
+struct Raw;  // 16 bytes of a row
+template <>
+struct Raw<float> {
+  static constexpr uint32_t kMasked = 0xff800000u;  // -inf
+  static __device__ __forceinline__ void unpack(const uint4& r, float* x) {
+    x[0] = __uint_as_float(r.x);
+    x[1] = __uint_as_float(r.y);
+    x[2] = __uint_as_float(r.z);
+    x[3] = __uint_as_float(r.w);
+  }
+  // Largest of the vectors' values, NaN ignored (NaN only if all are).
+  template <int U>
+  static __device__ __forceinline__ float vec_max(const uint4 (&r)[U]) {
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      m = fmaxf(fmaxf(fmaxf(__uint_as_float(r[u].x), __uint_as_float(r[u].y)),
+                      fmaxf(__uint_as_float(r[u].z), __uint_as_float(r[u].w))),
+                m);
+    return m;
+  }
+};
+
+// The same for two 16-bit values a word, compared in pairs.
+template <class T2, int U>
+__device__ __forceinline__ T2 packed_max(const uint4 (&r)[U]) {
+  auto as = [](const uint32_t& w) { return *reinterpret_cast<const T2*>(&w); };
+  T2 m = __hmax2(__hmax2(as(r[0].x), as(r[0].y)),
+                 __hmax2(as(r[0].z), as(r[0].w)));
+#pragma unroll
+  for (int u = 1; u < U; ++u)
+    m = __hmax2(m, __hmax2(__hmax2(as(r[u].x), as(r[u].y)),
+                           __hmax2(as(r[u].z), as(r[u].w))));
+  return m;
+}
+template <>
+struct Raw<__nv_bfloat16> {
+  static constexpr uint32_t kMasked = 0xff80ff80u;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* x) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  template <int U>
+  static __device__ __forceinline__ float vec_max(const uint4 (&r)[U]) {
+    const __nv_bfloat162 m = packed_max<__nv_bfloat162>(r);
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
+template <>
+struct Raw<__half> {
+  static constexpr uint32_t kMasked = 0xfc00fc00u;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* x) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  template <int U>
+  static __device__ __forceinline__ float vec_max(const uint4 (&r)[U]) {
+    const __half2 m = packed_max<__half2>(r);
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
+
+__device__ __forceinline__ uint4 load_16(const void* p) {
+  return __ldg(static_cast<const uint4*>(p));
+}
+
+// A vector at the edge of the row, element by element.
+template <class T>
+__device__ __forceinline__ uint4 edge_vec(const RowVecs<T>& rv, int vec) {
+  constexpr int E = RowVecs<T>::E;
+  uint4 r;
+  r.x = r.y = r.z = r.w = Raw<T>::kMasked;
+  T* t = reinterpret_cast<T*>(&r);
+  const int64_t i0 = rv.first(vec);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (i0 + e >= 0 && i0 + e < rv.v) t[e] = rv.row[i0 + e];
+  return r;
+}
+
+// Vector `vec` of the row, or -inf past `end`.
+template <class T>
+__device__ __forceinline__ uint4 load_vec(const RowVecs<T>& rv, int vec,
+                                          int end) {
+  uint4 r;
+  r.x = r.y = r.z = r.w = Raw<T>::kMasked;
+  if (vec < end) {
+    if (rv.inner(vec))
+      r = load_16(rv.row + rv.first(vec));
+    else
+      r = edge_vec(rv, vec);
+  }
+  return r;
+}
+
+// 2^x, 2 ulp (ex2.approx: 2^-22 relative, results below 2^-126 flushed).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)),
+        "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)),
+        "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+// log2(e) / T for 2^((l - m) * scale), finite for every T > 0 so that a
+// difference of 0 keeps weight 1.
+__device__ __forceinline__ float scale_of(float t) {
+  return fminf(static_cast<float>(1.4426950408889634074 /
+                                  static_cast<double>(t)),
+               3.402823466e38f);
+}
+
+// exp((l - m) / T) in fp32. Relative error: half a step each for l - m, the
+// product and the scale act on the exponent, 3 * 2^-24 * ln2 * |z|, z = the
+// exponent of 2; plus 2^-22 of ex2.
+__device__ __forceinline__ float weight32(float l, float m, float scale) {
+  if (l == m) return 1.0f;
+  if (!(l > -CUDART_INF_F)) return 0.0f;
+  return exp2_fast((l - m) * scale);
+}
+
+// ---------------------------------------------------------------------------
+// Drawing a token over a cluster, in 64 bits
+// ---------------------------------------------------------------------------
+constexpr int kCWarps = 8;  // of a block that draws
+constexpr int kCThreads = kCWarps * 32;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxSpans = 128;  // contiguous spans a row is cut into
+
+// The vectors [v0, v1) of a row in span `w` of `n`.
+struct Span {
+  int v0, v1;
+};
+__device__ __forceinline__ Span nth_span(int nv, int w, int per) {
+  Span s;
+  s.v0 = min(nv, w * per);
+  s.v1 = min(nv, s.v0 + per);
+  return s;
+}
+__device__ __forceinline__ Span span_of(int nv, int w, int n) {
+  return nth_span(nv, w, (nv + n - 1) / n);
+}
+
+// The span that holds u times the total of `spans` sums, sum_of(i) giving
+// them (called for lane * per + i): the first whose running sum exceeds the
+// target, else the last with mass, -1 without any; `ahead` is the sum in
+// front of it. The same in every lane of the warp.
+struct Pick {
+  int span;
+  double ahead;
+  double target;
+  double total;
+};
+template <class SumOf>
+__device__ __forceinline__ Pick pick_span(int spans, double u, SumOf sum_of) {
+  constexpr int kPer = kMaxSpans / 32;
+  const int per = (spans + 31) / 32;
+  double v[kPer];
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = lane_id() * per + i;
+    v[i] = i < per && at < spans ? sum_of(at) : 0.0;
+    sum += v[i];
+  }
+  double incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(SG_FULL_MASK, incl, o);
+    if (lane_id() >= o) incl += t;
+  }
+  Pick r;
+  r.total = __shfl_sync(SG_FULL_MASK, incl, 31);
+  r.target = u * r.total;
+  const unsigned over = __ballot_sync(SG_FULL_MASK, incl > r.target);
+  const unsigned has = __ballot_sync(SG_FULL_MASK, sum > 0.0);
+  r.span = -1;
+  r.ahead = 0.0;
+  if (has == 0) return r;
+  const int src = over ? __ffs(over) - 1 : 31 - __clz(has);
+  // within the lane: the first span that passes, else its last with mass
+  double run = incl - sum;
+  int at = -1;
+  double ahead = run;
+  bool done = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (!done && v[i] > 0.0) {
+      at = lane_id() * per + i;
+      ahead = run;
+      run += v[i];
+      done = run > r.target;
+    }
+  }
+  r.span = __shfl_sync(SG_FULL_MASK, at, src);
+  r.ahead = __shfl_sync(SG_FULL_MASK, ahead, src);
+  return r;
+}
+
+// The lowest index whose running sum of the source's weights exceeds u
+// times their total; the last one with a weight when rounding leaves none;
+// -1 without mass. Warps own contiguous spans over the cluster; the block
+// that owns the span with the target scans it. Called by every thread of
+// the cluster, same result in all.
+//   Src::E              weights of a vector
+//   src.nv              vectors
+//   src.first(v)        index of a vector's first weight
+//   src.sum(v, end, st) sum of the weights of vectors v, v + st, ... < end
+//   src.vec(v, end, w)  weights of vector v
+struct DrawShared {
+  double seg[kMaxCluster * kCWarps];
+  double red[32];
+  int32_t tok, first, last;
+};
+template <class Src>
+__device__ int32_t cluster_draw(const cooperative_groups::cluster_group& cl,
+                                const Src& src, double u, DrawShared& sh) {
+  constexpr int E = Src::E;
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int rank = static_cast<int>(cl.block_rank());
+  const int spans = cs * kCWarps;
+  const int mine = rank * kCWarps + warp_id();
+  const Span sp = span_of(src.nv, mine, spans);
+  const double s = warp_sum64(src.sum(sp.v0 + lane_id(), sp.v1, 32));
+  cl.sync();  // sh is free
+  if (lane_id() < cs) *cl.map_shared_rank(&sh.seg[mine], lane_id()) = s;
+  cl.sync();
+  const Pick pick = pick_span(spans, u, [&](int i) { return sh.seg[i]; });
+  if (pick.span < 0) return -1;
+  if (pick.span / kCWarps == rank) {
+    // a contiguous run of vectors a thread
+    const Span seg = span_of(src.nv, pick.span, spans);
+    const int per = (seg.v1 - seg.v0 + kCThreads - 1) / kCThreads;
+    const int v0 = min(seg.v1, seg.v0 + static_cast<int>(threadIdx.x) * per);
+    const int v1 = min(seg.v1, v0 + per);
+    const double mass = src.sum(v0, v1, 1);
+    double incl = mass;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(SG_FULL_MASK, incl, o);
+      if (lane_id() >= o) incl += t;
+    }
+    if (lane_id() == 31) sh.red[warp_id()] = incl;
+    if (threadIdx.x == 0) {
+      sh.first = INT32_MAX;
+      sh.last = -1;
+    }
+    __syncthreads();
+    double lo = pick.ahead;
+    for (int i = 0; i < warp_id(); ++i) lo += sh.red[i];
+    lo += incl - mass;
+    if (mass > 0.0 && !(lo > pick.target)) {  // or u is NaN
+      double run = lo;
+      int32_t at = -1;
+      bool over = false;
+      double w[E];
+      for (int v = v0; v < v1 && !over; ++v) {
+        src.vec(v, v1, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (!over && w[e] > 0.0) {
+            at = static_cast<int32_t>(src.first(v) + e);
+            run += w[e];
+            over = run > pick.target;
+          }
+        }
+      }
+      if (over)
+        atomicMin(&sh.first, at);
+      else
+        atomicMax(&sh.last, at);
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < cs)
+      *cl.map_shared_rank(&sh.tok, static_cast<int>(threadIdx.x)) =
+          sh.first != INT32_MAX ? sh.first : sh.last;
+  }
+  cl.sync();
+  return sh.tok;
 }
 
 }  // namespace sg

@@ -2,6 +2,9 @@
 // numbers) and from probabilities. Definitions in include/suffixgpu.h.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "sg_sampling.cuh"
 
 namespace sg {
@@ -271,6 +274,713 @@ __global__ void __launch_bounds__(kVThreads) pick_kernel(PickArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// verification from logits without filters
+// ---------------------------------------------------------------------------
+// Two launches. The first reads every row once, in spans (one a warp, `split`
+// blocks a row), and stores each span's largest value and the sum of its
+// weights relative to it. The second decides, a cluster a request, from the
+// spans' sums; it reads again only the span that holds the drawn token.
+//
+// Whether u < P(x) is decided from fp32 weights where u * Z and the weight
+// of x are further apart than their error can be (guard_of); otherwise the
+// row is summed again in 64 bits. The drawn token is found the same way:
+// in fp32 while the target lies clear of both borders of the token found,
+// else in 64 bits.
+constexpr int kSWarps = 8;  // warps of a block that reads rows
+constexpr int kSThreads = kSWarps * 32;
+constexpr int kMaxSplit = kMaxSpans / kSWarps;  // blocks that share a row
+constexpr int kSBlocks = 3;  // such blocks on an SM
+constexpr int kUnroll = 8;  // 16-byte loads in flight per thread
+
+struct Part {  // a span of a row
+  float s;     // sum of 2^((l - m) * scale)
+  float m;
+  int32_t arg;
+};
+
+struct VerifyArgs {
+  sg_rows rows;
+  sg_sampling set;
+  const int32_t* draft;
+  const int32_t* num_valid;
+  const float* uniforms;  // NULL: greedy
+  int32_t* sampled;
+  int32_t* count;
+  int32_t split;       // blocks that share a row
+  int32_t warp_spans;  // spans of each of their warps
+  double guard;   // relative error of sums of fp32 weights
+  Part* parts;    // [B * positions][split * kSWarps * warp_spans]
+  // many rows only (else NULL); zero at the start
+  int32_t* rejected;  // [B] positions - the lowest position known rejected
+  int32_t* arrived;   // [B * positions] blocks of the row that are done
+  int32_t* marks;     // requests to be decided by sums in 64 bits,
+  int32_t* marked;    // and which
+};
+
+// Largest value over the warp (-inf at least).
+__device__ __forceinline__ float warp_max(float m) {
+  return key_value(__reduce_max_sync(SG_FULL_MASK, order_key(m)));
+}
+
+// What a lane knows of its warp's span so far.
+struct LaneStat {
+  float m;      // the warp's largest value
+  double s;     // this lane's sum, relative to m
+  int32_t arg;  // lowest index of the largest value
+};
+
+// Takes U vectors a lane into `st`; index(u) is the row index of vector u's
+// first element. kArg: the lowest index of the largest value, looked for
+// where the vectors reach the block's largest so far (s_top); kSum: the
+// weights.
+template <class T, bool kArg, bool kSum, int U, class Index>
+__device__ __forceinline__ void take_vecs(const uint4 (&raw)[U], Index index,
+                                          float scale, uint32_t* s_top,
+                                          LaneStat& st) {
+  constexpr int E = RowVecs<T>::E;
+  const float tm = warp_max(canon(Raw<T>::vec_max(raw)));
+  bool up = kArg ? tm >= st.m && tm > -CUDART_INF_F : tm > st.m;
+  if (kArg && up) {
+    uint32_t old = 0;
+    if (lane_id() == 0) old = atomicMax(s_top, order_key(tm));
+    up = order_key(tm) >= __shfl_sync(SG_FULL_MASK, old, 0);
+  }
+  if (up) {
+    if (kSum && st.s != 0.0) st.s *= weight32(st.m, tm, scale);
+    if (kArg) {
+      int32_t at = tm == st.m ? st.arg : INT32_MAX;
+#pragma unroll
+      for (int u = U - 1; u >= 0; --u) {
+        float x[E];
+        Raw<T>::unpack(raw[u], x);
+        const int32_t i0 = static_cast<int32_t>(index(u));
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (x[e] == tm) at = min(at, i0 + e);
+      }
+      st.arg = __reduce_min_sync(SG_FULL_MASK, at);
+    }
+    st.m = tm;
+  }
+  if (kSum && st.m > -CUDART_INF_F) {
+    const float2 nm = make_float2(-st.m, -st.m);
+    const float2 sc = make_float2(scale, scale);
+    float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[E];
+      Raw<T>::unpack(raw[u], x);
+      float2 p[E / 2];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        p[e] = mul2(add2(make_float2(x[2 * e], x[2 * e + 1]), nm), sc);
+        p[e] = make_float2(exp2_fast(p[e].x), exp2_fast(p[e].y));
+      }
+#pragma unroll
+      for (int w = E / 4; w > 0; w /= 2)
+#pragma unroll
+        for (int e = 0; e < w; ++e) p[e] = add2(p[e], p[e + w]);
+      acc = add2(acc, p[0]);
+    }
+    float ts = acc.x + acc.y;
+    // NaN: masked NaN logits, +inf, or an infinite temperature's scale of 0
+    // on -inf; such vectors are summed again with each case told apart
+    if (ts != ts) {
+      ts = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[E];
+        Raw<T>::unpack(raw[u], x);
+        float us = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          us += weight32(canon(x[e]), st.m, scale);
+        ts += us;
+      }
+    }
+    st.s += ts;
+  }
+}
+
+// One warp's span of a row. The row's partial vectors at its two ends are
+// loaded first and taken last, so that they cost no latency of their own.
+template <class T, bool kArg, bool kSum>
+__device__ __forceinline__ Part warp_stats(const RowVecs<T>& rv, Span sp,
+                                           float scale, uint32_t* s_top) {
+  uint4 edge[1];
+  edge[0].x = edge[0].y = edge[0].z = edge[0].w = Raw<T>::kMasked;
+  const int ev = lane_id() == 0 ? sp.v0 : sp.v1 - 1;
+  const bool edges =
+      sp.v0 < sp.v1 && (!rv.inner(sp.v0) || !rv.inner(sp.v1 - 1));
+  if (edges && lane_id() < 2 && !rv.inner(ev) &&
+      (lane_id() == 0 || sp.v1 - 1 != sp.v0))
+    edge[0] = edge_vec(rv, ev);
+  LaneStat st{-CUDART_INF_F, 0.0, INT32_MAX};
+  for (int t0 = sp.v0; t0 < sp.v1; t0 += kUnroll * 32) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      raw[u].x = raw[u].y = raw[u].z = raw[u].w = Raw<T>::kMasked;
+      const int v = t0 + u * 32 + lane_id();
+      if (v < sp.v1 && rv.inner(v)) raw[u] = load_16(rv.row + rv.first(v));
+    }
+    take_vecs<T, kArg, kSum>(
+        raw, [&](int u) { return rv.first(t0 + u * 32 + lane_id()); }, scale,
+        s_top, st);
+  }
+  if (edges)
+    take_vecs<T, kArg, kSum>(
+        edge, [&](int) { return rv.first(ev); }, scale, s_top, st);
+  float s = 0.0f;
+  if (kSum) {
+    s = static_cast<float>(st.s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(SG_FULL_MASK, s, o);
+  }
+  return Part{s, st.m, st.arg};
+}
+
+// A row from the Parts of its `n` spans, in every lane of the warp.
+struct RowSum {
+  double s;
+  float m;
+  int32_t arg;
+};
+template <bool kArg, bool kSum>
+__device__ __forceinline__ RowSum join_parts(const Part* parts, int n,
+                                             float scale) {
+  constexpr int kPer = kMaxSpans / 32;
+  Part p[kPer];
+  float m = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    p[i] = Part{0.0f, -CUDART_INF_F, INT32_MAX};
+    if (i * 32 + lane_id() < n) p[i] = parts[i * 32 + lane_id()];
+    m = fmaxf(m, p[i].m);
+  }
+  RowSum r{0.0, warp_max(m), INT32_MAX};
+  int32_t arg = INT32_MAX;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (kSum && p[i].s != 0.0f)
+      r.s += static_cast<double>(p[i].s * weight32(p[i].m, r.m, scale));
+    if (kArg && p[i].m == r.m) arg = min(arg, p[i].arg);
+  }
+  if (kSum) r.s = warp_sum64(r.s);
+  if (kArg) r.arg = __reduce_min_sync(SG_FULL_MASK, arg);
+  return r;
+}
+
+// A weight's relative error is 3 * 2^-24 * ln2 = 1.24e-7 times its depth z
+// (its exponent of 2) plus 2^-22: at most kDeepGuard for one weight, whose
+// depth ends at 126. In a row's sum it counts by weight, and the weights'
+// mean depth is at most log2(V): it is their entropy less log2 of their sum,
+// and the largest weight is 1. Further errors: 2^-22 for each time the
+// largest value grew (at most once a tile) or spans were joined (2), and
+// 2^-24 for each of the at most 20 fp32 operations on a weight's way.
+constexpr double kDeepGuard = 1.7e-5;
+static double guard_of(int64_t vocab, int elems, int spans) {
+  const int64_t tile = static_cast<int64_t>(kUnroll) * 32 * elems;
+  const int64_t tiles = ceil_div(vocab, spans * tile) + 1;
+  return 1.25e-7 * std::log2(static_cast<double>(vocab) + 1.0) +
+         2.4e-7 * static_cast<double>(2 + tiles) + 1.2e-6;
+}
+
+// Spans of a warp, so that a span is one or two tiles.
+static int warp_spans_of(int64_t vocab, int elems, int split) {
+  const int64_t tile = static_cast<int64_t>(kUnroll) * 32 * elems;
+  const int64_t want = ceil_div(vocab, 2 * tile * split * kSWarps);
+  return static_cast<int>(
+      std::min<int64_t>(want, kMaxSpans / (split * kSWarps)));
+}
+
+// Whether a draft is accepted, where fp32 weights can tell.
+enum Verdict : int { kReject = 0, kAccept = 1, kUnsure = 2 };
+
+__device__ __forceinline__ Verdict verdict(const RowSum& row, float l, double u,
+                                           float scale, double guard) {
+  const double w = weight32(l, row.m, scale);
+  const double uz = u * row.s;
+  if (!(fabs(uz - w) > guard * uz + kDeepGuard * w)) return kUnsure;
+  return uz < w ? kAccept : kReject;
+}
+
+// One block's spans of row (b, j): block c's warps own a.warp_spans each.
+template <class T, bool kSampled>
+__device__ __forceinline__ void block_spans(const VerifyArgs& a, int b, int j,
+                                            int c, bool greedy, float scale,
+                                            uint32_t* s_top, Part* s_part) {
+  const RowVecs<T> rv(row_ptr<T>(a.rows, b, j), a.rows.vocab);
+  const int spans = a.split * kSWarps * a.warp_spans;
+  Part* out = a.parts +
+              (static_cast<int64_t>(b) * a.rows.positions + j) * spans;
+  const int per = (rv.nv + spans - 1) / spans;
+  for (int i = 0; i < a.warp_spans; ++i) {
+    const int at = warp_id() * a.warp_spans + i;  // in the block
+    const int w = c * kSWarps * a.warp_spans + at;
+    const Span sp = nth_span(rv.nv, w, per);
+    const Part p = greedy ? warp_stats<T, true, false>(rv, sp, scale, s_top)
+                          : warp_stats<T, false, true>(rv, sp, scale, s_top);
+    if (lane_id() == 0) {
+      out[w] = p;
+      s_part[at] = p;
+    }
+  }
+}
+
+// a.split blocks a row, the rows of low positions first. With many rows
+// (a.rejected), the last block of a row to arrive tells whether its draft is
+// surely rejected, and rows behind such a position are left out. What is
+// left out depends on timing; the rows that the decision reads do not.
+template <class T, bool kSampled>
+__global__ void __launch_bounds__(kSThreads, kSBlocks)
+    spans_kernel(VerifyArgs a) {
+  __shared__ Part s_part[kMaxSpans];
+  __shared__ uint32_t s_top;
+  __shared__ int32_t s_skip;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int k = a.rows.positions - 1;
+  const int c = static_cast<int>(blockIdx.x % a.split);
+  const int item = static_cast<int>(blockIdx.x / a.split);
+  const int b = item % a.rows.batch;
+  const int j = item / a.rows.batch;
+  if (threadIdx.x == 0) {
+    // read by one thread for the block: other blocks change it meanwhile
+    const int r = a.rejected
+        ? *static_cast<volatile int32_t*>(a.rejected + b) : 0;
+    s_skip = j > min(valid_drafts(a.num_valid, b, k), k + 1 - r);
+    s_top = 0;
+  }
+  __syncthreads();
+  if (s_skip) return;
+  Setting set{0.0f, 0, 1.0f};
+  if (kSampled) set = setting_of(a.set, b);
+  const bool greedy = !kSampled || !(set.t > 0.0f);
+  const float scale = greedy ? 0.0f : scale_of(set.t);
+  block_spans<T, kSampled>(a, b, j, c, greedy, scale, &s_top, s_part);
+  if (a.rejected == nullptr || j >= k) return;
+  if (a.split > 1 && lane_id() == 0) __threadfence();
+  __syncthreads();
+  if (warp_id() != 0) return;
+  const int64_t at = static_cast<int64_t>(b) * (k + 1) + j;
+  const int spans = a.split * kSWarps * a.warp_spans;
+  const Part* row_parts = s_part;
+  if (a.split > 1) {
+    int last = 0;
+    if (lane_id() == 0) last = atomicAdd(a.arrived + at, 1) == a.split - 1;
+    if (!__shfl_sync(SG_FULL_MASK, last, 0)) return;
+    __threadfence();
+    row_parts = a.parts + at * spans;
+  }
+  const RowSum r = greedy ? join_parts<true, false>(row_parts, spans, scale)
+                        : join_parts<false, true>(row_parts, spans, scale);
+  if (lane_id() != 0) return;
+  const int32_t x = a.draft[static_cast<int64_t>(b) * k + j];
+  bool reject = x < 0 || x >= a.rows.vocab || !(r.m > -CUDART_INF_F);
+  if (!reject) {
+    if (greedy) {
+      reject = x != r.arg;
+    } else {
+      const double u = a.uniforms[static_cast<int64_t>(b) * (k + 1) + j];
+      const float l = canon(to_f32(row_ptr<T>(a.rows, b, j)[x]));
+      reject = verdict(r, l, u, scale, a.guard) == kReject;
+    }
+  }
+  if (reject) atomicMax(a.rejected + b, k + 1 - j);
+}
+
+// A row's weights; `skip` (an index, or -1) has none.
+template <class T>
+struct RowWeights : RowVecs<T> {
+  using RowVecs<T>::E;
+  float m;
+  float scale;
+  double scale64;
+  int64_t skip;
+  const double* tab;
+
+  __device__ __forceinline__ RowWeights(const T* row, int64_t vocab, float m_,
+                                        float scale_, double scale64_,
+                                        int64_t skip_, const double* tab_)
+      : RowVecs<T>(row, vocab), m(m_), scale(scale_), scale64(scale64_),
+        skip(skip_), tab(tab_) {}
+
+  // fp32 weights of vector v; their sum.
+  __device__ __forceinline__ float fast_vec(int v, int end, float* w) const {
+    float x[E];
+    Raw<T>::unpack(load_vec(*this, v, end), x);
+    const int64_t i0 = this->first(v);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      w[e] = i0 + e == skip ? 0.0f : weight32(canon(x[e]), m, scale);
+    float s[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = w[e];
+#pragma unroll
+    for (int h = E / 2; h > 0; h /= 2)
+#pragma unroll
+      for (int e = 0; e < h; ++e) s[e] += s[e + h];
+    return s[0];
+  }
+
+  __device__ __forceinline__ void exact(const uint4& raw, int v,
+                                        double* w) const {
+    float x[E];
+    Raw<T>::unpack(raw, x);
+    if (m == CUDART_INF_F) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = x[e] == m ? 1.0 : 0.0;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = weight64(x[e], m, scale64, tab);
+    }
+    const int64_t at = skip - this->first(v);
+    if (at >= 0 && at < E) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e == at) w[e] = 0.0;
+    }
+  }
+  // Exact weights (cluster_draw's source).
+  __device__ __forceinline__ void vec(int v, int end, double* w) const {
+    exact(load_vec(*this, v, end), v, w);
+  }
+  __device__ __forceinline__ double sum(int v, int end, int step) const {
+    double s = 0.0;
+    if (v >= end) return s;
+    uint4 next = load_vec(*this, v, end);
+    for (; v < end; v += step) {
+      const uint4 raw = next;
+      next = load_vec(*this, v + step, end);  // in flight meanwhile
+      double w[E];
+      exact(raw, v, w);
+#pragma unroll
+      for (int h = E / 2; h > 0; h /= 2)
+#pragma unroll
+        for (int e = 0; e < h; ++e) w[e] += w[e + h];
+      s += w[0];
+    }
+    return s;
+  }
+};
+
+// Sum of a row's exact weights over the cluster, the same in every thread.
+template <class T>
+__device__ double cluster_sum64(const cooperative_groups::cluster_group& cl,
+                                const RowWeights<T>& weights,
+                                DrawShared& sh) {
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int rank = static_cast<int>(cl.block_rank());
+  const Span sp = span_of(weights.nv, rank * kCWarps + warp_id(),
+                          cs * kCWarps);
+  const double s = block_sum64(
+      weights.sum(sp.v0 + lane_id(), sp.v1, 32), sh.red);
+  cl.sync();  // sh.seg is free
+  if (static_cast<int>(threadIdx.x) < cs)
+    *cl.map_shared_rank(&sh.seg[rank], static_cast<int>(threadIdx.x)) = s;
+  cl.sync();
+  double z = 0.0;
+  for (int c = 0; c < cs; ++c) z += sh.seg[c];
+  cl.sync();  // and free again
+  return z;
+}
+
+// The token that cluster_draw gives, looked for in one span by the whole
+// block from fp32 weights: the span's running sums start `ahead` of the
+// row's; -2 when the target is nearer to a border of the token found than
+// `guard`.
+template <class T>
+__device__ int32_t span_draw(const RowWeights<T>& weights, Span sp,
+                             double ahead, double target, double guard,
+                             float* red, int32_t* s_found) {
+  constexpr int E = RowVecs<T>::E;
+  // a contiguous run of vectors a thread; exclusive sums over the block
+  const int per = (sp.v1 - sp.v0 + kCThreads - 1) / kCThreads;
+  const int v0 = min(sp.v1, sp.v0 + static_cast<int>(threadIdx.x) * per);
+  const int v1 = min(sp.v1, v0 + per);
+  float w[E];
+  double sum = 0.0;
+  for (int v = v0; v < v1; ++v) sum += weights.fast_vec(v, v1, w);
+  const float s = static_cast<float>(sum);
+  float incl = s;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float t = __shfl_up_sync(SG_FULL_MASK, incl, o);
+    if (lane_id() >= o) incl += t;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *s_found = -2;
+  if (lane_id() == 31) red[warp_id()] = incl;
+  __syncthreads();
+  float before = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kCWarps; ++i) before += i < warp_id() ? red[i] : 0.0f;
+  // at most one token is clear of both of its borders
+  const double need = target - ahead;
+  double lo = before + (incl - s);
+  if (need - lo > guard && lo + sum - need > guard) {
+    for (int v = v0; v < v1; ++v) {
+      weights.fast_vec(v, v1, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (need - lo > guard && lo + w[e] - need > guard)
+          *s_found = static_cast<int32_t>(weights.first(v) + e);
+        lo += w[e];
+      }
+    }
+  }
+  __syncthreads();
+  return *s_found;
+}
+
+// Every CTA of a request's cluster decides alike from the same numbers; the
+// cluster is needed where a row has to be summed in 64 bits. With many
+// requests that is left to a second launch: the first, a block a request,
+// only marks those that need it.
+enum Stage : int { kWhole, kMark, kMarked };
+
+struct DecideShared {
+  RowSum row[kCWarps];
+  int32_t x[kCWarps];
+  float l[kCWarps];
+  int32_t verdict[kCWarps];
+  DrawShared draw;
+  double tab[kExpTable];
+  float red[kCWarps];
+  int32_t found;
+};
+
+template <class T, bool kSampled, Stage kStage>
+__device__ void decide(const VerifyArgs& a,
+                       const cooperative_groups::cluster_group& cl, int b,
+                       bool leader, DecideShared& sh) {
+  const int k = a.rows.positions - 1;
+  const int64_t vocab = a.rows.vocab;
+  const int spans = a.split * kSWarps * a.warp_spans;
+  const int n = valid_drafts(a.num_valid, b, k);
+  const int32_t* drow = a.draft + static_cast<int64_t>(b) * k;
+  const float* urow = kSampled
+      ? a.uniforms + static_cast<int64_t>(b) * (k + 1) : nullptr;
+  int32_t* out = a.sampled + static_cast<int64_t>(b) * (k + 1);
+  if (n < 0) {
+    if (leader) emit(drow, 0, -1, k, out, a.count + b);
+    return;
+  }
+  const Setting set = kSampled ? setting_of(a.set, b)
+                               : Setting{0.0f, 0, 1.0f};
+  const bool greedy = !kSampled || !(set.t > 0.0f);
+  const float scale = greedy ? 0.0f : scale_of(set.t);
+  const double scale64 = greedy ? 0.0 : scale64_of(set.t);
+  const Part* parts = a.parts + static_cast<int64_t>(b) * (k + 1) * spans;
+
+  const auto mark = [&] {
+    if (threadIdx.x == 0) a.marked[atomicAdd(a.marks, 1)] = b;
+  };
+
+  // a warp a position, until one is not accepted; position n never is
+  int s = -1;
+  int32_t skip = -1;
+  float skip_l = 0.0f;
+  RowSum stop{};
+  for (int j0 = 0; s < 0; j0 += kCWarps) {
+    const int j = j0 + warp_id();
+    if (j <= n) {
+      int32_t x = -1;
+      float l = 0.0f;
+      double u = 0.0;
+      if (j < n) {
+        x = drow[j];
+        const T* r = row_ptr<T>(a.rows, b, j);
+        if (x < 0 || x >= vocab || r == nullptr) x = -1;
+        if (kSampled) u = urow[j];
+        if (!greedy && x >= 0) l = canon(to_f32(r[x]));
+      }
+      const Part* rp = parts + static_cast<int64_t>(j) * spans;
+      const RowSum row = greedy ? join_parts<true, false>(rp, spans, scale)
+                              : join_parts<false, true>(rp, spans, scale);
+      Verdict v = kReject;
+      if (x >= 0 && row.m > -CUDART_INF_F)
+        v = greedy ? (x == row.arg && u < 1.0 ? kAccept : kReject)
+                   : verdict(row, l, u, scale, a.guard);
+      if (lane_id() == 0) {
+        sh.row[warp_id()] = row;
+        sh.x[warp_id()] = x;
+        sh.l[warp_id()] = l;
+        sh.verdict[warp_id()] = v;
+      }
+    }
+    __syncthreads();
+    for (int g = 0; g < kCWarps && s < 0; ++g) {
+      int v = sh.verdict[g];
+      if (v == kUnsure) {
+        if (kStage == kMark) {
+          mark();
+          return;
+        }
+        const float m = sh.row[g].m;
+        const RowWeights<T> weights(row_ptr<T>(a.rows, b, j0 + g), vocab, m,
+                                    scale, scale64, -1, sh.tab);
+        const double z = cluster_sum64(cl, weights, sh.draw);
+        const double u = urow[j0 + g];
+        const double w = m == CUDART_INF_F
+            ? (sh.l[g] == m ? 1.0 : 0.0)
+            : weight64(sh.l[g], m, scale64, sh.tab);
+        v = u < w / z ? kAccept : kReject;
+      }
+      if (v == kReject) {
+        s = j0 + g;
+        stop = sh.row[g];
+        skip = s < n ? sh.x[g] : -1;
+        skip_l = sh.l[g];
+      }
+    }
+    __syncthreads();
+  }
+  int32_t tok = stop.m > -CUDART_INF_F ? stop.arg : -1;
+  if (!greedy && stop.m > -CUDART_INF_F) {
+    RowWeights<T> weights(row_ptr<T>(a.rows, b, s), vocab, stop.m, scale,
+                          scale64, skip, sh.tab);
+    const double u = urow[k];
+    // The span that holds the target, from the spans' sums; every warp
+    // finds it for itself. The rejected token's weight leaves its span.
+    const Part* rp = parts + static_cast<int64_t>(s) * spans;
+    const int skip_span =
+        skip < 0 ? -1
+                 : static_cast<int>((static_cast<int64_t>(skip) +
+                                     weights.head) / RowVecs<T>::E) /
+                       ((weights.nv + spans - 1) / spans);
+    const Pick pick = pick_span(spans, u, [&](int i) {
+      const Part p = rp[i];
+      double v = p.s == 0.0f ? 0.0f : p.s * weight32(p.m, stop.m, scale);
+      if (i == skip_span)
+        v = fmax(v - weight32(skip_l, stop.m, scale), 0.0);
+      return v;
+    });
+    tok = -2;
+    if (pick.span >= 0)
+      tok = span_draw(weights, span_of(weights.nv, pick.span, spans),
+                      pick.ahead, pick.target, stop.s * a.guard, sh.red,
+                      &sh.found);
+    if (kStage == kMark && tok == -2) {
+      mark();
+      return;
+    }
+    if (tok == -2) tok = cluster_draw(cl, weights, u, sh.draw);
+    if (tok < 0) {  // nothing but the rejected token
+      weights.skip = -1;
+      tok = cluster_draw(cl, weights, u, sh.draw);
+    }
+  }
+  if (leader) emit(drow, s, tok, k, out, a.count + b);
+}
+
+template <class T, bool kSampled, Stage kStage>
+__global__ void __launch_bounds__(kCThreads) decide_kernel(VerifyArgs a) {
+  const auto cl = cooperative_groups::this_cluster();
+  __shared__ DecideShared sh;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (kSampled) fill_exp_table(sh.tab);
+  __syncthreads();
+  const int cs = static_cast<int>(cl.num_blocks());
+  const bool leader = cl.block_rank() == 0;
+  const int first = static_cast<int>(blockIdx.x) / cs;
+  if (kStage != kMarked) {
+    decide<T, kSampled, kStage>(a, cl, first, leader, sh);
+    return;
+  }
+  // clusters take the marked requests in turns
+  const int marks = *a.marks;
+  for (int i = first; i < marks; i += static_cast<int>(gridDim.x) / cs) {
+    decide<T, kSampled, kStage>(a, cl, a.marked[i], leader, sh);
+    __syncthreads();
+  }
+}
+
+// A launch that may become resident while the previous kernel on the stream
+// finishes (it waits for that kernel before it reads anything).
+template <class Kernel>
+static int launch_after(Kernel* kernel, unsigned grid, int threads,
+                        int cluster, const VerifyArgs& a, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    cudaGetLastError();
+    return SG_ERR_CUDA;
+  }
+  return check_launch();
+}
+
+template <class T, bool kSampled>
+static int launch_verify_t(const VerifyArgs& a, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>(a.rows.batch) *
+                        static_cast<unsigned>(a.rows.positions) *
+                        static_cast<unsigned>(a.split);
+  int rc = launch_after(spans_kernel<T, kSampled>, grid, kSThreads, 1,
+                              a, st);
+  if (rc != SG_OK) return rc;
+  const unsigned requests = static_cast<unsigned>(a.rows.batch);
+  if constexpr (!kSampled) {
+    return launch_after(decide_kernel<T, false, kWhole>, requests, kCThreads,
+                        1, a, st);
+  } else {
+    if (a.marks == nullptr)
+      return launch_after(decide_kernel<T, true, kWhole>, requests * kMaxCluster,
+                          kCThreads, kMaxCluster, a, st);
+    rc = launch_after(decide_kernel<T, true, kMark>, requests, kCThreads, 1,
+                      a, st);
+    if (rc != SG_OK) return rc;
+    return launch_after(decide_kernel<T, true, kMarked>,
+                        std::min(requests, 74u) * kMaxCluster, kCThreads,
+                        kMaxCluster, a, st);
+  }
+}
+
+template <bool kSampled>
+static int launch_verify(const VerifyArgs& a, cudaStream_t st) {
+  switch (a.rows.dtype) {
+    case SG_F32:
+      return launch_verify_t<float, kSampled>(a, st);
+    case SG_BF16:
+      return launch_verify_t<__nv_bfloat16, kSampled>(a, st);
+    default:
+      return launch_verify_t<__half, kSampled>(a, st);
+  }
+}
+
+// With many rows (more than resident blocks) two blocks share a row: rows
+// read in vain before a rejection is known get fewer than with one (256 x 17
+// rows of 128256 bf16: 78 us against 87; with four the blocks that find
+// nothing to do outweigh that, 80 us).
+constexpr int kManySplit = 2;
+
+// Up to this batch one launch with a cluster a request decides everything
+// (64 requests without drafts: 24 us against 35 with the second launch;
+// 256 requests: 65 against 50).
+constexpr int kWholeBatch = 128;
+
+// Blocks that share a row: enough to fill the machine's resident blocks.
+static int split_of(int64_t rows) {
+  const int64_t s = rows > 0 ? kSBlocks * 148 / rows : 1;
+  return static_cast<int>(std::min<int64_t>(kMaxSplit,
+                                            std::max<int64_t>(1, s)));
+}
+
+// ---------------------------------------------------------------------------
 // verification from probabilities: one block a request
 // ---------------------------------------------------------------------------
 struct ProbArgs {
@@ -421,14 +1131,61 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
     return SG_ERR_INVALID;
   rc = check_workspace(logits, workspace, workspace_bytes);
   if (rc != SG_OK) return rc;
+  if (static_cast<int64_t>(logits->batch) * logits->positions >
+      INT32_MAX / kMaxSplit)
+    return SG_ERR_UNSUPPORTED;
+  const bool filtered =
+      sampling && (sampling->top_k || sampling->top_p ||
+                   sampling->top_k_all > 0 || sampling->top_p_all < 1.0f);
+  if (!filtered) {
+    VerifyArgs va{};
+    va.rows = *logits;
+    if (sampling) va.set = *sampling;
+    va.draft = draft;
+    va.num_valid = num_valid;
+    va.uniforms = uniforms;
+    va.sampled = sampled;
+    va.count = count;
+    const int64_t rows =
+        static_cast<int64_t>(logits->batch) * logits->positions;
+    va.split = split_of(rows);
+    const bool many = va.split == 1 && logits->positions > 1;
+    if (many) va.split = kManySplit;
+    va.parts = static_cast<Part*>(workspace);
+    const int elems = logits->dtype == SG_F32 ? 4 : 8;
+    va.warp_spans = warp_spans_of(logits->vocab, elems, va.split);
+    const int spans = va.split * kSWarps * va.warp_spans;
+    va.guard = guard_of(logits->vocab, elems, spans);
+    int32_t* ctl = reinterpret_cast<int32_t*>(va.parts + rows * spans);
+    size_t zero = 0;
+    if (sampling && logits->batch > kWholeBatch) {
+      va.marks = ctl;
+      va.marked = ctl + 1 + logits->batch + rows;
+      zero = 1;
+    }
+    if (many) {
+      va.rejected = ctl + 1;
+      va.arrived = va.rejected + logits->batch;
+      zero = 1 + logits->batch + rows;
+    }
+    if (zero) {
+      const cudaError_t err = cudaMemsetAsync(ctl, 0, zero * sizeof(int32_t), st);
+      if (err != cudaSuccess) {
+        set_cuda_error(err);
+        return SG_ERR_CUDA;
+      }
+    }
+    return sampling ? launch_verify<true>(va, st)
+                    : launch_verify<false>(va, st);
+  }
   StatArgs sa{};
   sa.rows = *logits;
-  if (sampling) sa.set = *sampling;
+  sa.set = *sampling;
   sa.draft = draft;
   sa.num_valid = num_valid;
   sa.uniforms = uniforms;
   sa.stats = static_cast<RowStat*>(workspace);
-  rc = sampling ? launch_stats<false>(sa, st) : launch_stats<true>(sa, st);
+  rc = launch_stats<false>(sa, st);
   if (rc != SG_OK) return rc;
   return launch_pick(PickArgs{*logits, sa.set, sa.stats, draft, num_valid,
                               uniforms, sampled, count},
@@ -440,9 +1197,11 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
 using namespace sg;
 
 extern "C" size_t sg_verify_workspace_size(int32_t batch, int32_t positions) {
-  if (batch < 0 || positions < 0) return 0;
-  return static_cast<size_t>(batch) * static_cast<size_t>(positions) *
-         sizeof(RowStat);
+  if (batch <= 0 || positions <= 0) return 0;
+  const size_t rows = static_cast<size_t>(batch) * positions;
+  const size_t spans = rows * kMaxSpans * sizeof(Part) +
+      (1 + 2 * static_cast<size_t>(batch) + rows) * sizeof(int32_t);
+  return std::max(spans, rows * sizeof(RowStat));
 }
 
 extern "C" int sg_verify_greedy(const sg_rows* logits, const int32_t* draft,
