@@ -690,11 +690,11 @@ __device__ double cluster_sum64(const cooperative_groups::cluster_group& cl,
 // block from fp32 weights: the span's running sums start `ahead` of the
 // row's; -2 when the target is nearer to a border of the token found than
 // `guard`.
-template <class T>
-__device__ int32_t span_draw(const RowWeights<T>& weights, Span sp,
-                             double ahead, double target, double guard,
-                             float* red, int32_t* s_found) {
-  constexpr int E = RowVecs<T>::E;
+template <class W>
+__device__ int32_t span_draw(const W& weights, Span sp, double ahead,
+                             double target, double guard, float* red,
+                             int32_t* s_found) {
+  constexpr int E = W::E;
   // a contiguous run of vectors a thread; exclusive sums over the block
   const int per = (sp.v1 - sp.v0 + kCThreads - 1) / kCThreads;
   const int v0 = min(sp.v1, sp.v0 + static_cast<int>(threadIdx.x) * per);
@@ -900,9 +900,9 @@ __global__ void __launch_bounds__(kCThreads) decide_kernel(VerifyArgs a) {
 
 // A launch that may become resident while the previous kernel on the stream
 // finishes (it waits for that kernel before it reads anything).
-template <class Kernel>
-static int launch_after(Kernel* kernel, unsigned grid, int threads,
-                        int cluster, const VerifyArgs& a, cudaStream_t st) {
+template <class Args>
+static int launch_after(void (*kernel)(Args), unsigned grid, int threads,
+                        int cluster, const Args& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -975,14 +975,21 @@ constexpr int kWholeBatch = 128;
 
 // Blocks that share a row: enough to fill the machine's resident blocks.
 static int split_of(int64_t rows) {
-  const int64_t s = rows > 0 ? kSBlocks * 148 / rows : 1;
+  const int64_t s = rows > 0 ? (kSBlocks * 148 + rows / 2) / rows : 1;
   return static_cast<int>(std::min<int64_t>(kMaxSplit,
                                             std::max<int64_t>(1, s)));
 }
 
 // ---------------------------------------------------------------------------
-// verification from probabilities: one block a request
+// verification from probabilities: one cluster a request
 // ---------------------------------------------------------------------------
+// The acceptance tests are K gathers, which every block of the cluster makes
+// for itself; then the one row the token is drawn from (and the drafter's)
+// is read once, split over the cluster. Its sums are fp32 over a few
+// vectors and 64 bits beyond; where the target is not clear of the borders
+// of the token found, the row is summed again with every weight in 64 bits
+// (differences of fp32 probabilities are exact there). Converting every
+// value to 64 bits in the first place took twice the time of its bytes.
 struct ProbArgs {
   sg_rows p;
   sg_rows q;
@@ -994,23 +1001,196 @@ struct ProbArgs {
   int32_t* count;
 };
 
-__global__ void __launch_bounds__(kVThreads) probs_kernel(ProbArgs a) {
-  __shared__ double seg[32];
+// max(p - q, 0) (q NULL: p), without token `skip`: cluster_draw's source.
+struct ProbWeights : RowVecs<float> {
+  const float* q;
+  bool q_vecs;  // q's rows lie on the same 16-byte grid as p's
+  int64_t skip;
+
+  __device__ __forceinline__ ProbWeights(const float* p, const float* q_,
+                                         int64_t vocab, int64_t skip_)
+      : RowVecs<float>(p, vocab), q(q_), skip(skip_) {
+    q_vecs = ((reinterpret_cast<uintptr_t>(p) ^
+               reinterpret_cast<uintptr_t>(q_)) & 15) == 0;
+  }
+  __device__ __forceinline__ uint4 load(const float* row, int vec,
+                                        bool vecs) const {
+    uint4 r;
+    r.x = r.y = r.z = r.w = 0;
+    const int64_t i0 = first(vec);
+    if (vecs && inner(vec)) return load_16(row + i0);
+    if (i0 >= 0 && i0 < v) r.x = __float_as_uint(row[i0]);
+    if (i0 + 1 >= 0 && i0 + 1 < v) r.y = __float_as_uint(row[i0 + 1]);
+    if (i0 + 2 >= 0 && i0 + 2 < v) r.z = __float_as_uint(row[i0 + 2]);
+    if (i0 + 3 >= 0 && i0 + 3 < v) r.w = __float_as_uint(row[i0 + 3]);
+    return r;
+  }
+  __device__ __forceinline__ double weight(uint32_t a, uint32_t b) const {
+    const double d =
+        static_cast<double>(clean_prob(__uint_as_float(a))) -
+        static_cast<double>(clean_prob(__uint_as_float(b)));
+    return d > 0.0 ? d : 0.0;
+  }
+  __device__ __forceinline__ void weights(const uint4& a, const uint4& b,
+                                          int vec, double* w) const {
+    w[0] = weight(a.x, b.x);
+    w[1] = weight(a.y, b.y);
+    w[2] = weight(a.z, b.z);
+    w[3] = weight(a.w, b.w);
+    const int64_t at = skip - first(vec);
+    if (at >= 0 && at < E) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e == at) w[e] = 0.0;
+    }
+  }
+  __device__ __forceinline__ void vec(int at, int end, double* w) const {
+    uint4 a, b;
+    a.x = a.y = a.z = a.w = 0;
+    b = a;
+    if (at < end) {
+      a = load(row, at, true);
+      if (q) b = load(q, at, q_vecs);
+    }
+    weights(a, b, at, w);
+  }
+  // fp32 weights of a vector; their sum. A weight is off by 2^-24 of it; an
+  // infinite p gives an infinite sum, which no token is clear of.
+  __device__ __forceinline__ float fast(const uint4& a, const uint4& b,
+                                        int vec, float* w) const {
+    const uint32_t pa[E] = {a.x, a.y, a.z, a.w};
+    const uint32_t qa[E] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      w[e] = fmaxf(__uint_as_float(pa[e]), 0.0f);
+      if (q) w[e] = fmaxf(w[e] - clean_prob(__uint_as_float(qa[e])), 0.0f);
+    }
+    const int64_t at = skip - first(vec);
+    if (at >= 0 && at < E) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e == at) w[e] = 0.0f;
+    }
+    return (w[0] + w[1]) + (w[2] + w[3]);
+  }
+  __device__ __forceinline__ float fast_vec(int at, int end, float* w) const {
+    uint4 a, b;
+    a.x = a.y = a.z = a.w = 0;
+    b = a;
+    if (at < end) {
+      a = load(row, at, true);
+      if (q) b = load(q, at, q_vecs);
+    }
+    return fast(a, b, at, w);
+  }
+  __device__ __forceinline__ double fast_sum(int at, int end, int step) const {
+    constexpr int U = 4;  // loads in flight
+    double s = 0.0;
+    for (; at < end; at += U * step) {
+      uint4 a[U], b[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        a[u].x = a[u].y = a[u].z = a[u].w = 0;
+        b[u] = a[u];
+        const int i = at + u * step;
+        if (i < end) {
+          a[u] = load(row, i, true);
+          if (q) b[u] = load(q, i, q_vecs);
+        }
+      }
+      float t[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float w[E];
+        t[u] = fast(a[u], b[u], at + u * step, w);
+      }
+#pragma unroll
+      for (int h = U / 2; h > 0; h /= 2)
+#pragma unroll
+        for (int u = 0; u < h; ++u) t[u] += t[u + h];
+      s += t[0];
+    }
+    return s;
+  }
+  __device__ __forceinline__ double sum(int at, int end, int step) const {
+    constexpr int U = 4;  // loads of each row in flight
+    double s = 0.0;
+    for (; at < end; at += U * step) {
+      uint4 a[U], b[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        a[u].x = a[u].y = a[u].z = a[u].w = 0;
+        b[u] = a[u];
+        const int i = at + u * step;
+        if (i < end) {
+          a[u] = load(row, i, true);
+          if (q) b[u] = load(q, i, q_vecs);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        double w[E];
+        weights(a[u], b[u], at + u * step, w);
+        s += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+    }
+    return s;
+  }
+};
+
+// The fp32 additions on a weight's way (at most 17) and its own rounding.
+constexpr double kProbGuard = 1.2e-6;
+
+// cluster_draw from fp32 sums; -2 where they cannot tell.
+__device__ int32_t cluster_try_draw(
+    const cooperative_groups::cluster_group& cl, const ProbWeights& weights,
+    double u, DrawShared& sh, float* red, int32_t* s_found) {
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int rank = static_cast<int>(cl.block_rank());
+  const int spans = cs * kCWarps;
+  const int mine = rank * kCWarps + warp_id();
+  const Span sp = span_of(weights.nv, mine, spans);
+  const double s = warp_sum64(weights.fast_sum(sp.v0 + lane_id(), sp.v1, 32));
+  cl.sync();  // every block runs before any writes into another
+  if (lane_id() < cs) *cl.map_shared_rank(&sh.seg[mine], lane_id()) = s;
+  cl.sync();
+  const Pick pick = pick_span(spans, u, [&](int i) { return sh.seg[i]; });
+  if (pick.span < 0) return -1;
+  if (pick.span / kCWarps == rank) {
+    const int32_t tok =
+        span_draw(weights, span_of(weights.nv, pick.span, spans), pick.ahead,
+                  pick.target, pick.total * kProbGuard, red, s_found);
+    if (static_cast<int>(threadIdx.x) < cs)
+      *cl.map_shared_rank(&sh.tok, static_cast<int>(threadIdx.x)) = tok;
+  }
+  cl.sync();
+  return sh.tok;
+}
+
+__global__ void __launch_bounds__(kCThreads, 5) probs_kernel(ProbArgs a) {
+  const auto cl = cooperative_groups::this_cluster();
+  __shared__ DrawShared sh;
+  __shared__ float s_red[kCWarps];
+  __shared__ int32_t s_found;
   __shared__ int s_stop;
-  const int b = blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int b = static_cast<int>(blockIdx.x) / cs;
+  const bool leader = cl.block_rank() == 0;
   const int k = a.p.positions - 1;
   const int64_t v = a.p.vocab;
   const int n = valid_drafts(a.num_valid, b, k);
   const int32_t* drow = a.draft + static_cast<int64_t>(b) * k;
   const float* u = a.uniforms + static_cast<int64_t>(b) * (k + 1);
   int32_t* out = a.sampled + static_cast<int64_t>(b) * (k + 1);
-  if (n < 0) {
-    emit(drow, 0, -1, k, out, a.count + b);
+  if (n < 0) {  // the whole cluster leaves: no barrier is waited for
+    if (leader) emit(drow, 0, -1, k, out, a.count + b);
     return;
   }
   if (threadIdx.x == 0) s_stop = n;
   __syncthreads();
-  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+  for (int j = threadIdx.x; j < n; j += kCThreads) {
     const int32_t x = drow[j];
     const float* prow = row_ptr<float>(a.p, b, j);
     bool ok = false;
@@ -1026,26 +1206,16 @@ __global__ void __launch_bounds__(kVThreads) probs_kernel(ProbArgs a) {
   const float* prow = row_ptr<float>(a.p, b, s);
   int32_t tok = -1;
   if (prow != nullptr) {
-    auto p_of = [&](int64_t i) {
-      return static_cast<double>(clean_prob(prow[i]));
-    };
-    if (s < n && a.has_q) {
-      const float* qrow = row_ptr<float>(a.q, b, s);
-      tok = block_draw(
-          v, u[k],
-          [&](int64_t i) {
-            return fmax(p_of(i) - static_cast<double>(clean_prob(qrow[i])),
-                        0.0);
-          },
-          seg);
-    } else if (s < n) {
-      const int64_t x = drow[s];
-      tok = block_draw(
-          v, u[k], [&](int64_t i) { return i == x ? 0.0 : p_of(i); }, seg);
-    }
-    if (tok < 0) tok = block_draw(v, u[k], p_of, seg);
+    const float* qrow =
+        s < n && a.has_q ? row_ptr<float>(a.q, b, s) : nullptr;
+    const int64_t skip = s < n && !a.has_q ? drow[s] : -1;
+    const ProbWeights weights(prow, qrow, v, skip);
+    tok = cluster_try_draw(cl, weights, u[k], sh, s_red, &s_found);
+    if (tok == -2) tok = cluster_draw(cl, weights, u[k], sh);
+    if (tok < 0 && s < n)  // nothing left: the row itself
+      tok = cluster_draw(cl, ProbWeights(prow, nullptr, v, -1), u[k], sh);
   }
-  emit(drow, s, tok, k, out, a.count + b);
+  if (leader) emit(drow, s, tok, k, out, a.count + b);
 }
 
 // ---------------------------------------------------------------------------
@@ -1149,7 +1319,7 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
     const int64_t rows =
         static_cast<int64_t>(logits->batch) * logits->positions;
     va.split = split_of(rows);
-    const bool many = va.split == 1 && logits->positions > 1;
+    const bool many = rows > kSBlocks * 148 && logits->positions > 1;
     if (many) va.split = kManySplit;
     va.parts = static_cast<Part*>(workspace);
     const int elems = logits->dtype == SG_F32 ? 4 : 8;
@@ -1258,9 +1428,11 @@ extern "C" int sg_verify_probs(const sg_rows* probs,
   a.uniforms = uniforms;
   a.sampled = sampled;
   a.count = count;
-  probs_kernel<<<static_cast<unsigned>(probs->batch), kVThreads, 0,
-                 reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  return check_launch();
+  if (probs->batch > INT32_MAX / kMaxCluster) return SG_ERR_UNSUPPORTED;
+  return launch_after(probs_kernel,
+                      static_cast<unsigned>(probs->batch) * kMaxCluster,
+                      kCThreads, kMaxCluster, a,
+                      reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int sg_target_probs(const sg_rows* logits,
