@@ -253,8 +253,7 @@ typedef struct sg_sampling {
   int32_t pad_;
 } sg_sampling;
 
-/* Workspace bytes of sg_verify_greedy, sg_verify_sampled and
- * sg_target_probs. Calls that may overlap on the GPU (other streams, other
+/* Workspace bytes of sg_verify_greedy and sg_verify_sampled. Calls that may overlap on the GPU (other streams, other
  * graphs) need workspaces of their own. */
 size_t sg_verify_workspace_size(int32_t batch, int32_t positions);
 
@@ -284,10 +283,11 @@ int sg_verify_probs(const sg_rows* probs, const sg_rows* draft_probs,
                     sg_stream_t stream);
 
 /* The target's probabilities P of every row, out [B, positions, V] fp32
- * (contiguous). */
+ * (contiguous). Here and in sg_verify_sampled with top-k or top-p, a row has
+ * to fit the shared memory of 8 SMs: SG_ERR_UNSUPPORTED beyond about 1.3 MB
+ * (a vocabulary of 350 thousand in fp32). */
 int sg_target_probs(const sg_rows* logits, const sg_sampling* sampling,
-                    float* out, void* workspace, size_t workspace_bytes,
-                    sg_stream_t stream);
+                    float* out, sg_stream_t stream);
 
 /* ---- vLLM glue ----------------------------------------------------------- */
 

@@ -164,8 +164,7 @@ _SIGS: dict[str, list] = {
                           c_size_t, c_void_p],
     "sg_verify_probs": [POINTER(Rows), POINTER(Rows), c_void_p, c_void_p,
                         c_void_p, c_void_p, c_void_p, c_void_p],
-    "sg_target_probs": [POINTER(Rows), POINTER(Sampling), c_void_p, c_void_p,
-                        c_size_t, c_void_p],
+    "sg_target_probs": [POINTER(Rows), POINTER(Sampling), c_void_p, c_void_p],
     "sg_global_combine": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                           c_void_p, c_void_p, c_int32, c_int32, c_int32,
                           c_void_p],

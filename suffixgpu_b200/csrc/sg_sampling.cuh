@@ -16,10 +16,10 @@ namespace sg {
 // statistics kernels and read by the kernels that pick or write.
 struct RowStat {
   double z;       // sum of the kept weights, relative to the largest value
-  float m;        // largest value of the row (-inf: no mass)
-  int32_t arg;    // its lowest index (-1: no mass)
-  uint32_t tkey;  // order key of the smallest kept value
-  int32_t accept; // 1: this position's draft is accepted
+  float m;         // largest value of the row
+  int32_t arg;     // its lowest index (greedy rows), -1: no mass
+  float low;       // smallest kept value
+  int32_t accept;  // 1: this position's draft is accepted
 };
 
 // Row `j` of request `b`, or null when the request has no such row.
@@ -53,14 +53,6 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-
-// exp((l - m) / T) in 64 bits; inv_t = 1 / T. A row with +inf entries gives
-// them equal shares; -inf has no weight under any temperature.
-__device__ __forceinline__ double weight64(float l, float m, double inv_t) {
-  if (l == m) return 1.0;
-  if (l == -CUDART_INF_F || m == CUDART_INF_F) return 0.0;
-  return exp((static_cast<double>(l) - static_cast<double>(m)) * inv_t);
 }
 
 // Exact weights: exp((l - m) / T) in 64 bits without branches, so that the
@@ -110,6 +102,11 @@ __device__ __forceinline__ float clean_prob(float p) {
   return (p > 0.0f && p < CUDART_INF_F) ? p : 0.0f;
 }
 
+// Largest value over the warp (-inf at least).
+__device__ __forceinline__ float warp_max(float m) {
+  return key_value(__reduce_max_sync(SG_FULL_MASK, order_key(m)));
+}
+
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(SG_FULL_MASK, v, o);
@@ -148,6 +145,46 @@ __device__ __forceinline__ Setting setting_of(const sg_sampling& s, int b) {
   r.k = s.top_k ? s.top_k[b] : s.top_k_all;
   r.p = s.top_p ? s.top_p[b] : s.top_p_all;
   return r;
+}
+
+inline bool has_filter(const sg_sampling& s) {
+  return s.top_k || s.top_p || s.top_k_all > 0 || s.top_p_all < 1.0f;
+}
+
+// Statistics of the rows that a verification with top-k or top-p reads
+// (target_probs.cu). rejected [B] and *taken are zero at the start.
+int launch_row_stats(const sg_rows& rows, const sg_sampling& set,
+                     const int32_t* draft, const int32_t* num_valid,
+                     const float* uniforms, RowStat* stats, int32_t* rejected,
+                     int32_t* taken, cudaStream_t st);
+
+// A launch that may become resident while the previous kernel on the stream
+// finishes (it waits for that kernel before it reads anything).
+template <class Args>
+inline int launch_after(void (*kernel)(Args), unsigned grid, int threads,
+                        int cluster, const Args& a, cudaStream_t st,
+                        size_t smem = 0) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    cudaGetLastError();
+    return SG_ERR_CUDA;
+  }
+  return check_launch();
 }
 
 // Host-side checks of a row set; batch and positions may be 0.

@@ -610,10 +610,9 @@ at::Tensor target_probs(const at::Tensor& logits,
   const c10::cuda::CUDAGuard guard(rows.device());
   r.data = rows.data_ptr();
   at::Tensor out = at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
-  at::Tensor ws = verify_workspace(r, rows);
   check_status("sg_target_probs",
-               sg_target_probs(&r, &s, out.data_ptr<float>(), ws.data_ptr(),
-                               ws.numel(), stream_for(rows)));
+               sg_target_probs(&r, &s, out.data_ptr<float>(),
+                               stream_for(rows)));
   return out;
 }
 

@@ -9,210 +9,6 @@
 
 namespace sg {
 
-constexpr int kVThreads = 512;
-
-// ---------------------------------------------------------------------------
-// statistics: one block a row
-// ---------------------------------------------------------------------------
-struct StatArgs {
-  sg_rows rows;
-  sg_sampling set;
-  const int32_t* draft;      // [B, K] or NULL (statistics only)
-  const int32_t* num_valid;  // [B] or NULL
-  const float* uniforms;     // [B, K + 1] or NULL (greedy)
-  RowStat* stats;            // [B * positions]
-};
-
-template <class T>
-__device__ __forceinline__ float value_at(const T* row, int64_t i) {
-  return canon(to_f32(row[i]));
-}
-
-// Largest value and its lowest index, in every thread.
-template <class T>
-__device__ void block_argmax(const T* row, int64_t v, float* m_out,
-                             int32_t* arg_out) {
-  __shared__ float s_m[32];
-  __shared__ int32_t s_i[32];
-  float m = -CUDART_INF_F;
-  int32_t arg = INT32_MAX;
-  for (int64_t i = threadIdx.x; i < v; i += blockDim.x) {
-    const float x = value_at(row, i);
-    if (x > m) {
-      m = x;
-      arg = static_cast<int32_t>(i);
-    }
-  }
-  for (int pass = 0; pass < 2; ++pass) {
-    if (pass == 1) {
-      __syncthreads();
-      if (lane_id() == 0) {
-        s_m[warp_id()] = m;
-        s_i[warp_id()] = arg;
-      }
-      __syncthreads();
-      const bool in = lane_id() < static_cast<int>(blockDim.x >> 5);
-      m = in ? s_m[lane_id()] : -CUDART_INF_F;
-      arg = in ? s_i[lane_id()] : INT32_MAX;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float om = __shfl_xor_sync(SG_FULL_MASK, m, o);
-      const int32_t oi = __shfl_xor_sync(SG_FULL_MASK, arg, o);
-      if (om > m || (om == m && oi < arg)) {
-        m = om;
-        arg = oi;
-      }
-    }
-  }
-  *m_out = m;
-  *arg_out = m > -CUDART_INF_F ? arg : -1;
-}
-
-template <class T, bool kGreedy>
-__global__ void __launch_bounds__(kVThreads) row_stats_kernel(StatArgs a) {
-  __shared__ double red[32];
-  const int b = blockIdx.x % a.rows.batch;
-  const int j = blockIdx.x / a.rows.batch;
-  const int k = a.rows.positions - 1;
-  int n = k;
-  if (a.draft != nullptr || k == 0) {
-    n = valid_drafts(a.num_valid, b, k);
-    if (j > n) return;
-  }
-  RowStat* out = a.stats + static_cast<int64_t>(b) * a.rows.positions + j;
-  const T* row = row_ptr<T>(a.rows, b, j);
-  const int64_t v = a.rows.vocab;
-  RowStat st;
-  st.z = 0.0;
-  st.m = -CUDART_INF_F;
-  st.arg = -1;
-  st.tkey = 0;
-  st.accept = 0;
-  if (row != nullptr) block_argmax(row, v, &st.m, &st.arg);
-  Setting set{0.0f, 0, 1.0f};
-  if (!kGreedy) set = setting_of(a.set, b);
-  const bool greedy = kGreedy || !(set.t > 0.0f);
-  if (!greedy && st.arg >= 0) {
-    const double inv_t = 1.0 / static_cast<double>(set.t);
-    // top-k: the largest key held by at least k tokens from it on
-    uint32_t low = 0;
-    if (set.k > 0 && set.k < v) {
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t cand = low | (1u << bit);
-        int c = 0;
-        for (int64_t i = threadIdx.x; i < v; i += blockDim.x)
-          c += order_key(value_at(row, i)) >= cand;
-        if (block_sum64(c, red) >= set.k) low = cand;
-      }
-    }
-    auto mass = [&](uint32_t from) {
-      double s = 0.0;
-      for (int64_t i = threadIdx.x; i < v; i += blockDim.x) {
-        const float x = value_at(row, i);
-        if (order_key(x) >= from) s += weight64(x, st.m, inv_t);
-      }
-      return block_sum64(s, red);
-    };
-    if (set.p < 1.0f) {
-      if (set.p > 0.0f) {
-        const double need = static_cast<double>(set.p) * mass(low);
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-          const uint32_t cand = t | (1u << bit);
-          if (mass(max(cand, low)) >= need) t = cand;
-        }
-        low = max(low, t);
-      } else {
-        low = order_key(st.m);
-      }
-    }
-    st.tkey = low;
-    st.z = mass(low);
-  }
-  if (threadIdx.x == 0) {
-    if (a.draft != nullptr && j < n) {
-      const int32_t x = a.draft[static_cast<int64_t>(b) * k + j];
-      if (x >= 0 && x < v && st.arg >= 0) {
-        const double u = a.uniforms
-            ? static_cast<double>(
-                  a.uniforms[static_cast<int64_t>(b) * (k + 1) + j])
-            : 0.0;
-        if (greedy) {
-          st.accept = x == st.arg && u < 1.0;
-        } else {
-          const float l = value_at(row, x);
-          const double w = order_key(l) >= st.tkey
-              ? weight64(l, st.m, 1.0 / static_cast<double>(set.t)) : 0.0;
-          st.accept = u < w / st.z;
-        }
-      }
-    }
-    *out = st;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// drawing one token from a row of weights
-// ---------------------------------------------------------------------------
-// The lowest i < v whose running sum of weight(i) exceeds u times the sum;
-// the last i with a weight when rounding leaves none; -1 without mass. A
-// warp owns a contiguous segment of the row. Same result in every thread.
-template <class W>
-__device__ int32_t block_draw(int64_t v, double u, W weight, double* seg) {
-  __shared__ int32_t s_tok;
-  const int warps = blockDim.x >> 5;
-  const int64_t len = ceil_div(ceil_div(v, warps), 32) * 32;
-  const int64_t lo = min(v, warp_id() * len);
-  const int64_t hi = min(v, lo + len);
-  double s = 0.0;
-  for (int64_t i = lo + lane_id(); i < hi; i += 32) s += weight(i);
-  s = warp_sum64(s);
-  __syncthreads();
-  if (threadIdx.x == 0) s_tok = -1;
-  if (lane_id() == 0) seg[warp_id()] = s;
-  __syncthreads();
-  double total = 0.0;
-  for (int w = 0; w < warps; ++w) total += seg[w];
-  const double target = u * total;
-  double before = 0.0;
-  int pick = -1;
-  for (int w = 0; w < warps; ++w) {
-    if (seg[w] > 0.0) pick = w;
-    if (before + seg[w] > target) break;
-    before += seg[w];
-  }
-  if (pick == warp_id()) {
-    // `before` covers the segments ahead of the one that passes the target;
-    // when none passes (rounding), the last segment with mass is scanned
-    double run = 0.0;
-    for (int w = 0; w < pick; ++w) run += seg[w];
-    int32_t tok = -1;
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-      const int64_t i = i0 + lane_id();
-      const double w = i < hi ? weight(i) : 0.0;
-      double incl = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double t = __shfl_up_sync(SG_FULL_MASK, incl, o);
-        if (lane_id() >= o) incl += t;
-      }
-      const unsigned has = __ballot_sync(SG_FULL_MASK, w > 0.0);
-      const unsigned over =
-          __ballot_sync(SG_FULL_MASK, w > 0.0 && run + incl > target);
-      if (has) tok = static_cast<int32_t>(i0 + 31 - __clz(has));
-      if (over) {
-        tok = static_cast<int32_t>(i0 + __ffs(over) - 1);
-        break;
-      }
-      run += __shfl_sync(SG_FULL_MASK, incl, 31);
-    }
-    if (lane_id() == 0) s_tok = tok;
-  }
-  __syncthreads();
-  return s_tok;
-}
-
 // Writes a request's ids and count: the first s drafts and the token after
 // them (-1: none).
 __device__ __forceinline__ void emit(const int32_t* drow, int s, int32_t tok,
@@ -220,57 +16,6 @@ __device__ __forceinline__ void emit(const int32_t* drow, int s, int32_t tok,
   for (int j = threadIdx.x; j <= k; j += blockDim.x)
     out[j] = j < s ? drow[j] : (j == s ? tok : -1);
   if (threadIdx.x == 0) *count = s + (tok >= 0 ? 1 : 0);
-}
-
-// ---------------------------------------------------------------------------
-// picking from logits: one block a request
-// ---------------------------------------------------------------------------
-struct PickArgs {
-  sg_rows rows;
-  sg_sampling set;
-  const RowStat* stats;
-  const int32_t* draft;
-  const int32_t* num_valid;
-  const float* uniforms;  // NULL: greedy
-  int32_t* sampled;
-  int32_t* count;
-};
-
-template <class T>
-__global__ void __launch_bounds__(kVThreads) pick_kernel(PickArgs a) {
-  __shared__ double seg[32];
-  const int b = blockIdx.x;
-  const int k = a.rows.positions - 1;
-  const int n = valid_drafts(a.num_valid, b, k);
-  const int32_t* drow = a.draft + static_cast<int64_t>(b) * k;
-  int32_t* out = a.sampled + static_cast<int64_t>(b) * (k + 1);
-  if (n < 0) {
-    emit(drow, 0, -1, k, out, a.count + b);
-    return;
-  }
-  const RowStat* stats = a.stats + static_cast<int64_t>(b) * (k + 1);
-  int s = 0;
-  while (s < n && stats[s].accept) ++s;
-  const RowStat st = stats[s];
-  int32_t tok = st.arg;
-  if (a.uniforms != nullptr && st.arg >= 0) {
-    const Setting set = setting_of(a.set, b);
-    if (set.t > 0.0f) {
-      const T* row = row_ptr<T>(a.rows, b, s);
-      const double inv_t = 1.0 / static_cast<double>(set.t);
-      const double u = a.uniforms[static_cast<int64_t>(b) * (k + 1) + k];
-      const int64_t out_tok = s < n ? drow[s] : -1;
-      auto weight = [&](int64_t i) {
-        const float x = value_at(row, i);
-        return order_key(x) >= st.tkey ? weight64(x, st.m, inv_t) : 0.0;
-      };
-      tok = block_draw(
-          a.rows.vocab, u,
-          [&](int64_t i) { return i == out_tok ? 0.0 : weight(i); }, seg);
-      if (tok < 0) tok = block_draw(a.rows.vocab, u, weight, seg);
-    }
-  }
-  emit(drow, s, tok, k, out, a.count + b);
 }
 
 // ---------------------------------------------------------------------------
@@ -316,11 +61,6 @@ struct VerifyArgs {
   int32_t* marks;     // requests to be decided by sums in 64 bits,
   int32_t* marked;    // and which
 };
-
-// Largest value over the warp (-inf at least).
-__device__ __forceinline__ float warp_max(float m) {
-  return key_value(__reduce_max_sync(SG_FULL_MASK, order_key(m)));
-}
 
 // What a lane knows of its warp's span so far.
 struct LaneStat {
@@ -898,33 +638,6 @@ __global__ void __launch_bounds__(kCThreads) decide_kernel(VerifyArgs a) {
   }
 }
 
-// A launch that may become resident while the previous kernel on the stream
-// finishes (it waits for that kernel before it reads anything).
-template <class Args>
-static int launch_after(void (*kernel)(Args), unsigned grid, int threads,
-                        int cluster, const Args& a, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    cudaGetLastError();
-    return SG_ERR_CUDA;
-  }
-  return check_launch();
-}
-
 template <class T, bool kSampled>
 static int launch_verify_t(const VerifyArgs& a, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>(a.rows.batch) *
@@ -978,6 +691,134 @@ static int split_of(int64_t rows) {
   const int64_t s = rows > 0 ? (kSBlocks * 148 + rows / 2) / rows : 1;
   return static_cast<int>(std::min<int64_t>(kMaxSplit,
                                             std::max<int64_t>(1, s)));
+}
+
+// ---------------------------------------------------------------------------
+// verification from logits with top-k or top-p
+// ---------------------------------------------------------------------------
+// The rows' statistics hold the smallest kept value, the kept mass and the
+// verdict on each draft (target_probs.cu); one cluster a request draws.
+struct PickArgs {
+  sg_rows rows;
+  sg_sampling set;
+  const RowStat* stats;
+  const int32_t* draft;
+  const int32_t* num_valid;
+  const float* uniforms;
+  int32_t* sampled;
+  int32_t* count;
+};
+
+// Exact weights of the values >= low, without token `skip`; weights are
+// formed only where a vector holds such a value.
+template <class T>
+struct KeptWeights : RowVecs<T> {
+  using RowVecs<T>::E;
+  float m, low;
+  double scale64;
+  int64_t skip;
+  const double* tab;
+
+  __device__ __forceinline__ KeptWeights(const T* row, int64_t vocab)
+      : RowVecs<T>(row, vocab) {}
+  __device__ __forceinline__ bool exact(const uint4& raw, int v,
+                                        double* w) const {
+    float x[E];
+    Raw<T>::unpack(raw, x);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) any = any || x[e] >= low;
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = 0.0;
+    if (!any) return false;
+    const int64_t i0 = this->first(v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (x[e] >= low && i0 + e != skip)
+        w[e] = x[e] == m ? 1.0
+                         : weight64(x[e], static_cast<double>(m), scale64,
+                                    tab);
+    }
+    return true;
+  }
+  __device__ __forceinline__ void vec(int v, int end, double* w) const {
+    exact(load_vec(*this, v, end), v, w);
+  }
+  __device__ __forceinline__ double sum(int v, int end, int step) const {
+    constexpr int U = 4;  // loads in flight
+    double s = 0.0;
+    for (; v < end; v += U * step) {
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = load_vec(*this, v + u * step, end);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        double w[E];
+        if (exact(raw[u], v + u * step, w)) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) s += w[e];
+        }
+      }
+    }
+    return s;
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kCThreads) pick_kernel(PickArgs a) {
+  const auto cl = cooperative_groups::this_cluster();
+  __shared__ DrawShared sh;
+  __shared__ double s_tab[kExpTable];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  fill_exp_table(s_tab);
+  __syncthreads();
+  const int b = static_cast<int>(blockIdx.x / cl.num_blocks());
+  const bool leader = cl.block_rank() == 0;
+  const int k = a.rows.positions - 1;
+  const int n = valid_drafts(a.num_valid, b, k);
+  const int32_t* drow = a.draft + static_cast<int64_t>(b) * k;
+  int32_t* out = a.sampled + static_cast<int64_t>(b) * (k + 1);
+  if (n < 0) {  // the whole cluster leaves: no barrier is waited for
+    if (leader) emit(drow, 0, -1, k, out, a.count + b);
+    return;
+  }
+  const RowStat* stats = a.stats + static_cast<int64_t>(b) * (k + 1);
+  int s = 0;
+  for (int j0 = 0;; j0 += 32) {
+    const int j = j0 + lane_id();
+    const unsigned no =
+        __ballot_sync(SG_FULL_MASK, j >= n || !stats[j].accept);
+    if (no) {
+      s = j0 + __ffs(no) - 1;
+      break;
+    }
+  }
+  const RowStat st = stats[s];
+  int32_t tok = st.arg;
+  const Setting set = setting_of(a.set, b);
+  if (st.arg >= 0 && set.t > 0.0f) {
+    const double u = a.uniforms[static_cast<int64_t>(b) * (k + 1) + k];
+    KeptWeights<T> weights(row_ptr<T>(a.rows, b, s), a.rows.vocab);
+    weights.m = st.m;
+    weights.low = st.low;
+    weights.scale64 = scale64_of(set.t);
+    weights.skip = s < n ? drow[s] : -1;
+    weights.tab = s_tab;
+    tok = cluster_draw(cl, weights, u, sh);
+    if (tok < 0) {  // nothing but the rejected token
+      weights.skip = -1;
+      tok = cluster_draw(cl, weights, u, sh);
+    }
+  }
+  if (leader) emit(drow, s, tok, k, out, a.count + b);
+}
+
+template <class T>
+static int launch_pick(const PickArgs& a, cudaStream_t st) {
+  return launch_after(pick_kernel<T>,
+                      static_cast<unsigned>(a.rows.batch) * kMaxCluster,
+                      kCThreads, kMaxCluster, a, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -1218,74 +1059,11 @@ __global__ void __launch_bounds__(kCThreads, 5) probs_kernel(ProbArgs a) {
   if (leader) emit(drow, s, tok, k, out, a.count + b);
 }
 
-// ---------------------------------------------------------------------------
-// probabilities of every row
-// ---------------------------------------------------------------------------
-template <class T>
-__global__ void __launch_bounds__(kVThreads)
-    write_probs_kernel(sg_rows rows, sg_sampling sampling,
-                       const RowStat* stats, float* out) {
-  const int b = blockIdx.x % rows.batch;
-  const int j = blockIdx.x / rows.batch;
-  const int64_t at = static_cast<int64_t>(b) * rows.positions + j;
-  const RowStat st = stats[at];
-  const T* row = row_ptr<T>(rows, b, j);
-  const Setting set = setting_of(sampling, b);
-  const double inv_t = 1.0 / static_cast<double>(set.t);
-  float* orow = out + at * rows.vocab;
-  for (int64_t i = threadIdx.x; i < rows.vocab; i += blockDim.x) {
-    float p = 0.0f;
-    if (st.arg >= 0) {
-      if (!(set.t > 0.0f)) {
-        p = i == st.arg ? 1.0f : 0.0f;
-      } else {
-        const float x = value_at(row, i);
-        if (order_key(x) >= st.tkey)
-          p = static_cast<float>(weight64(x, st.m, inv_t) / st.z);
-      }
-    }
-    orow[i] = p;
-  }
-}
-
 static int check_workspace(const sg_rows* r, const void* ws, size_t bytes) {
   const size_t need = sg_verify_workspace_size(r->batch, r->positions);
   if (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15))
     return SG_ERR_WORKSPACE;
   return SG_OK;
-}
-
-template <bool kGreedy>
-static int launch_stats(const StatArgs& a, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(a.rows.batch) * a.rows.positions;
-  if (rows > INT32_MAX) return SG_ERR_UNSUPPORTED;
-  const unsigned grid = static_cast<unsigned>(rows);
-  switch (a.rows.dtype) {
-    case SG_F32:
-      row_stats_kernel<float, kGreedy><<<grid, kVThreads, 0, st>>>(a);
-      break;
-    case SG_BF16:
-      row_stats_kernel<__nv_bfloat16, kGreedy><<<grid, kVThreads, 0, st>>>(a);
-      break;
-    default:
-      row_stats_kernel<__half, kGreedy><<<grid, kVThreads, 0, st>>>(a);
-  }
-  return check_launch();
-}
-
-static int launch_pick(const PickArgs& a, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>(a.rows.batch);
-  switch (a.rows.dtype) {
-    case SG_F32:
-      pick_kernel<float><<<grid, kVThreads, 0, st>>>(a);
-      break;
-    case SG_BF16:
-      pick_kernel<__nv_bfloat16><<<grid, kVThreads, 0, st>>>(a);
-      break;
-    default:
-      pick_kernel<__half><<<grid, kVThreads, 0, st>>>(a);
-  }
-  return check_launch();
 }
 
 static int verify(const sg_rows* logits, const sg_sampling* sampling,
@@ -1304,10 +1082,7 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
   if (static_cast<int64_t>(logits->batch) * logits->positions >
       INT32_MAX / kMaxSplit)
     return SG_ERR_UNSUPPORTED;
-  const bool filtered =
-      sampling && (sampling->top_k || sampling->top_p ||
-                   sampling->top_k_all > 0 || sampling->top_p_all < 1.0f);
-  if (!filtered) {
+  if (!sampling || !has_filter(*sampling)) {
     VerifyArgs va{};
     va.rows = *logits;
     if (sampling) va.set = *sampling;
@@ -1348,18 +1123,27 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
     return sampling ? launch_verify<true>(va, st)
                     : launch_verify<false>(va, st);
   }
-  StatArgs sa{};
-  sa.rows = *logits;
-  sa.set = *sampling;
-  sa.draft = draft;
-  sa.num_valid = num_valid;
-  sa.uniforms = uniforms;
-  sa.stats = static_cast<RowStat*>(workspace);
-  rc = launch_stats<false>(sa, st);
+  // rows' statistics, then [B] rejected positions and the rows handed out
+  RowStat* stats = static_cast<RowStat*>(workspace);
+  const int64_t rows = static_cast<int64_t>(logits->batch) * logits->positions;
+  int32_t* rejected = reinterpret_cast<int32_t*>(stats + rows);
+  const cudaError_t err = cudaMemsetAsync(
+      rejected, 0, (static_cast<size_t>(logits->batch) + 1) * sizeof(int32_t),
+      st);
+  if (err != cudaSuccess) {
+    set_cuda_error(err);
+    return SG_ERR_CUDA;
+  }
+  rc = launch_row_stats(*logits, *sampling, draft, num_valid, uniforms, stats,
+                        rejected, rejected + logits->batch, st);
   if (rc != SG_OK) return rc;
-  return launch_pick(PickArgs{*logits, sa.set, sa.stats, draft, num_valid,
-                              uniforms, sampled, count},
-                     st);
+  const PickArgs pa{*logits,   *sampling, stats,   draft,
+                    num_valid, uniforms,  sampled, count};
+  switch (logits->dtype) {
+    case SG_F32: return launch_pick<float>(pa, st);
+    case SG_BF16: return launch_pick<__nv_bfloat16>(pa, st);
+    default: return launch_pick<__half>(pa, st);
+  }
 }
 
 }  // namespace sg
@@ -1371,7 +1155,9 @@ extern "C" size_t sg_verify_workspace_size(int32_t batch, int32_t positions) {
   const size_t rows = static_cast<size_t>(batch) * positions;
   const size_t spans = rows * kMaxSpans * sizeof(Part) +
       (1 + 2 * static_cast<size_t>(batch) + rows) * sizeof(int32_t);
-  return std::max(spans, rows * sizeof(RowStat));
+  const size_t stats = rows * sizeof(RowStat) +
+                       (static_cast<size_t>(batch) + 1) * sizeof(int32_t);
+  return std::max(spans, stats);
 }
 
 extern "C" int sg_verify_greedy(const sg_rows* logits, const int32_t* draft,
@@ -1433,41 +1219,4 @@ extern "C" int sg_verify_probs(const sg_rows* probs,
                       static_cast<unsigned>(probs->batch) * kMaxCluster,
                       kCThreads, kMaxCluster, a,
                       reinterpret_cast<cudaStream_t>(stream));
-}
-
-extern "C" int sg_target_probs(const sg_rows* logits,
-                               const sg_sampling* sampling, float* out,
-                               void* workspace, size_t workspace_bytes,
-                               sg_stream_t stream) {
-  NvtxScope nvtx("sg_target_probs");
-  int rc = check_rows(logits, false);
-  if (rc != SG_OK) return rc;
-  if (!sampling || logits->row_start) return SG_ERR_INVALID;
-  if (logits->batch == 0 || logits->positions == 0) return SG_OK;
-  if (!out) return SG_ERR_INVALID;
-  rc = check_workspace(logits, workspace, workspace_bytes);
-  if (rc != SG_OK) return rc;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  StatArgs sa{};
-  sa.rows = *logits;
-  sa.set = *sampling;
-  sa.stats = static_cast<RowStat*>(workspace);
-  rc = launch_stats<false>(sa, st);
-  if (rc != SG_OK) return rc;
-  const unsigned grid = static_cast<unsigned>(
-      static_cast<int64_t>(logits->batch) * logits->positions);
-  switch (logits->dtype) {
-    case SG_F32:
-      write_probs_kernel<float><<<grid, kVThreads, 0, st>>>(
-          *logits, *sampling, sa.stats, out);
-      break;
-    case SG_BF16:
-      write_probs_kernel<__nv_bfloat16><<<grid, kVThreads, 0, st>>>(
-          *logits, *sampling, sa.stats, out);
-      break;
-    default:
-      write_probs_kernel<__half><<<grid, kVThreads, 0, st>>>(
-          *logits, *sampling, sa.stats, out);
-  }
-  return check_launch();
 }

@@ -198,13 +198,12 @@ def test_refused_at_the_c_abi():
     half = _lib.Rows(**{**ok, "dtype": 1})
     assert L.sg_verify_probs(ctypes.byref(half), None, one, None, one, one,
                              one, None) == 4
-    assert L.sg_target_probs(ctypes.byref(r), ctypes.byref(s), None, one,
-                             1 << 20, None) == 1
-    assert L.sg_target_probs(ctypes.byref(r), ctypes.byref(s), one, one, 8,
-                             None) == 2
+    assert L.sg_target_probs(ctypes.byref(r), ctypes.byref(s), None,
+                             None) == 1
+    assert L.sg_target_probs(ctypes.byref(r), None, one, None) == 1
     packed = _lib.Rows(**{**ok, "row_start": one, "n_rows": 6})
-    assert L.sg_target_probs(ctypes.byref(packed), ctypes.byref(s), one, one,
-                             1 << 20, None) == 1
+    assert L.sg_target_probs(ctypes.byref(packed), ctypes.byref(s), one,
+                             None) == 1
 
 
 def test_drafter_verify_refuses_settings_without_uniforms():
