@@ -206,7 +206,8 @@ int sg_expand_chain(const int32_t* cont, int32_t rows, int32_t max_occ,
  *   whose tokens >= t hold at least p of the kept mass (p <= 0: the largest
  *   value only), so tokens of one value stay or go together;
  *   P_i = w_i / the sum of the kept weights.
- *   T not > 0: P is 1 at the first largest token. A row whose entries are
+ *   T not > 0: P is 1 at the first largest token. (Positive T below the
+ *   smallest normal fp32 number counts as that.) A row whose entries are
  *   all -inf has no mass: P = 0.
  * Draft j (j < n = min(num_valid, K)) with token x is accepted while
  * 0 <= x < V and u_j * q_j(x) < P_j(x) (q = 1 where drafts come without

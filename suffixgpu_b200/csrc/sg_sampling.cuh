@@ -142,6 +142,7 @@ struct Setting {
 __device__ __forceinline__ Setting setting_of(const sg_sampling& s, int b) {
   Setting r;
   r.t = s.temperature ? s.temperature[b] : s.temperature_all;
+  if (r.t > 0.0f) r.t = fmaxf(r.t, 1.17549435e-38f);  // 1 / T stays finite
   r.k = s.top_k ? s.top_k[b] : s.top_k_all;
   r.p = s.top_p ? s.top_p[b] : s.top_p_all;
   return r;
@@ -366,12 +367,9 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&r);
 }
 
-// log2(e) / T for 2^((l - m) * scale), finite for every T > 0 so that a
-// difference of 0 keeps weight 1.
+// log2(e) / T for 2^((l - m) * scale); finite (see setting_of).
 __device__ __forceinline__ float scale_of(float t) {
-  return fminf(static_cast<float>(1.4426950408889634074 /
-                                  static_cast<double>(t)),
-               3.402823466e38f);
+  return static_cast<float>(1.4426950408889634074 / static_cast<double>(t));
 }
 
 // exp((l - m) / T) in fp32. Relative error: half a step each for l - m, the
@@ -381,6 +379,155 @@ __device__ __forceinline__ float weight32(float l, float m, float scale) {
   if (l == m) return 1.0f;
   if (!(l > -CUDART_INF_F)) return 0.0f;
   return exp2_fast((l - m) * scale);
+}
+
+// The scale in two parts, so that its rounding, which would act on all
+// weights alike and shift a row's probabilities by 2^-24 times their mean
+// depth, does not count: z = d * (hi + lo) is rounded once, by itself. hi is
+// rounded down and lo above 0, so that -inf keeps its sign.
+struct FineScale {
+  float hi, lo;
+};
+__device__ __forceinline__ FineScale fine_scale_of(float t) {
+  FineScale f;
+  const double s = 1.4426950408889634074 / static_cast<double>(t);
+  f.hi = __double2float_rd(s);
+  f.lo = fmaxf(static_cast<float>(s - static_cast<double>(f.hi)), 1e-30f);
+  return f;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)),
+        "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+// Weights of two values; NaN for NaN, and for m = +inf.
+__device__ __forceinline__ float2 fine_weight2(float2 l, float m,
+                                               const FineScale& f) {
+  const float2 d = add2(l, make_float2(-m, -m));
+  const float2 z = fma2(d, make_float2(f.hi, f.hi),
+                        mul2(d, make_float2(f.lo, f.lo)));
+  return make_float2(exp2_fast(z.x), exp2_fast(z.y));
+}
+
+// ---------------------------------------------------------------------------
+// One pass over values: largest and sum of weights
+// ---------------------------------------------------------------------------
+// What a lane knows of its warp's span so far.
+struct LaneStat {
+  float m;      // the warp's largest value
+  double s;     // this lane's sum, relative to m
+  int32_t arg;  // lowest index of the largest value
+};
+
+// Takes U vectors a lane into `st`; index(u) is the row index of vector u's
+// first element. kArg: the lowest index of the largest value, looked for
+// where the vectors reach the block's largest so far (s_top); kSum: the
+// weights' sum, from fp32 weights or finer ones.
+enum SumKind : int { kNoSum, kFastSum, kFineSum };
+
+template <class T, bool kArg, SumKind kSum, int U, class Index>
+__device__ __forceinline__ void take_vecs(const uint4 (&raw)[U], Index index,
+                                          const FineScale& f,
+                                          uint32_t* s_top, LaneStat& st) {
+  const float scale = f.hi;
+  constexpr int E = RowVecs<T>::E;
+  const float tm = warp_max(canon(Raw<T>::vec_max(raw)));
+  bool up = kArg ? tm >= st.m && tm > -CUDART_INF_F : tm > st.m;
+  if (kArg && up) {
+    uint32_t old = 0;
+    if (lane_id() == 0) old = atomicMax(s_top, order_key(tm));
+    up = order_key(tm) >= __shfl_sync(SG_FULL_MASK, old, 0);
+  }
+  if (up) {
+    if (kSum != kNoSum && st.s != 0.0) st.s *= weight32(st.m, tm, scale);
+    if (kArg) {
+      int32_t at = tm == st.m ? st.arg : INT32_MAX;
+#pragma unroll
+      for (int u = U - 1; u >= 0; --u) {
+        float x[E];
+        Raw<T>::unpack(raw[u], x);
+        const int32_t i0 = static_cast<int32_t>(index(u));
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (x[e] == tm) at = min(at, i0 + e);
+      }
+      st.arg = __reduce_min_sync(SG_FULL_MASK, at);
+    }
+    st.m = tm;
+  }
+  if (kSum != kNoSum && st.m > -CUDART_INF_F) {
+    const float2 nm = make_float2(-st.m, -st.m);
+    const float2 sc = make_float2(scale, scale);
+    float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[E];
+      Raw<T>::unpack(raw[u], x);
+      float2 p[E / 2];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        p[e] = make_float2(x[2 * e], x[2 * e + 1]);
+        if (kSum == kFineSum) {
+          p[e] = fine_weight2(p[e], st.m, f);
+        } else {
+          p[e] = mul2(add2(p[e], nm), sc);
+          p[e] = make_float2(exp2_fast(p[e].x), exp2_fast(p[e].y));
+        }
+      }
+#pragma unroll
+      for (int w = E / 4; w > 0; w /= 2)
+#pragma unroll
+        for (int e = 0; e < w; ++e) p[e] = add2(p[e], p[e + w]);
+      acc = add2(acc, p[0]);
+    }
+    float ts = acc.x + acc.y;
+    // NaN: masked NaN logits, +inf, or an infinite temperature's scale of 0
+    // on -inf; such vectors are summed again with each case told apart
+    if (ts != ts) {
+      ts = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[E];
+        Raw<T>::unpack(raw[u], x);
+        float us = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          us += weight32(canon(x[e]), st.m, scale);
+        ts += us;
+      }
+    }
+    st.s += ts;
+  }
+}
+
+// Sums over parts of a row, relative to the parts' largest values.
+struct SpanSum {
+  double s;
+  float m;
+  int32_t arg;
+};
+
+// The row's from those of its n <= 32 parts, in every lane of the warp; with
+// factors in 64 bits (t > 0; else only m and arg count).
+__device__ __forceinline__ SpanSum join_sums(const SpanSum* parts, int n,
+                                             float t) {
+  SpanSum p{0.0, -CUDART_INF_F, INT32_MAX};
+  if (lane_id() < n) p = parts[lane_id()];
+  const float m = warp_max(p.m);
+  p.arg = __reduce_min_sync(SG_FULL_MASK, p.m == m ? p.arg : INT32_MAX);
+  double s = 0.0;
+  if (p.s != 0.0 && t > 0.0f)
+    s = p.m == m ? p.s
+                 : p.s * exp((static_cast<double>(p.m) -
+                              static_cast<double>(m)) /
+                             static_cast<double>(t));
+  p.s = warp_sum64(s);
+  p.m = m;
+  return p;
 }
 
 // ---------------------------------------------------------------------------

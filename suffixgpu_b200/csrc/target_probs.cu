@@ -4,7 +4,6 @@
 //
 // One cluster a row; each block keeps its share of the row in shared memory,
 // so that the row is read from HBM once whatever the number of passes.
-// Clusters are resident and take rows one after another.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -15,6 +14,8 @@ namespace sg {
 
 constexpr int kFThreads = 256;
 constexpr int kFWarps = kFThreads / 32;
+constexpr int kSoftBlocks = 5;  // blocks on an SM, plain softmax
+constexpr int kKeptBlocks = 3;  // and with filters
 constexpr int kBins = 2048;
 constexpr int kList = 2048;      // candidates the first block can hold
 constexpr int kOwn = kList / kFThreads;
@@ -483,10 +484,10 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
 // ---------------------------------------------------------------------------
 // a row's statistics
 // ---------------------------------------------------------------------------
-template <class T, bool kFilter>
+template <class T>
 __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
                          Share<T>& sh, uint4* buf, const Setting& set,
-                         RowShared& rs, FilterShared* fs) {
+                         RowShared& rs, FilterShared& fs) {
   constexpr int U = 8;
   const int cs = static_cast<int>(cl.num_blocks());
   const int rank = static_cast<int>(cl.block_rank());
@@ -496,8 +497,7 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
   sh.v0 = sp.v0;
   sh.n = sp.v1 - sp.v0;
   sh.tab = rs.tab;
-  if (kFilter)
-    for (int i = tid; i < kBins; i += kFThreads) fs->hist[i] = 0;
+  for (int i = tid; i < kBins; i += kFThreads) fs.hist[i] = 0;
   float m = -CUDART_INF_F;
   for (int i0 = tid; i0 < sh.n; i0 += U * kFThreads) {
     uint4 raw[U];
@@ -539,9 +539,9 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
   }
   sh.scale = scale_of(set.t);
   sh.scale64 = scale64_of(set.t);
-  const int32_t k = kFilter && set.k > 0 && set.k < sh.v ? set.k : 0;
-  const float p = kFilter && set.p < 1.0f ? set.p : 1.0f;
-  if (kept.m == CUDART_INF_F || (kFilter && !(p > 0.0f))) {
+  const int32_t k = set.k > 0 && set.k < sh.v ? set.k : 0;
+  const float p = set.p < 1.0f ? set.p : 1.0f;
+  if (kept.m == CUDART_INF_F || !(p > 0.0f)) {
     // only the largest value has mass, or is kept
     int32_t c = 0;
     sh.each([&](float x, int64_t) { c += x == kept.m; });
@@ -552,10 +552,10 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
     kept.low = kept.m;
     return kept;
   }
-  if (kFilter && (k > 0 || p < 1.0f)) {
-    filter_row(cl, sh, k, p, rs, *fs);
-    kept.low = fs->low;
-    kept.z = fs->z;
+  if (k > 0 || p < 1.0f) {
+    filter_row(cl, sh, k, p, rs, fs);
+    kept.low = fs.low;
+    kept.z = fs.z;
     return kept;
   }
   double s = 0.0;
@@ -585,47 +585,172 @@ struct RowArgs {
 
 extern __shared__ uint4 row_smem[];
 
-template <class T, bool kFilter>
-__global__ void __launch_bounds__(kFThreads)
-    write_rows_kernel(RowArgs a) {
+// Eight (or, at odd places, single) probabilities.
+__device__ __forceinline__ void store_8(float* p, const float (&x)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p),
+               "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]),
+               "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
+
+// Writes a block's share of a row, f(pair of values) giving the
+// probabilities: vectors whole where the output lies on the vectors' grid,
+// else value by value (neighbouring threads on neighbouring values).
+template <class T, class F>
+__device__ __forceinline__ void write_share(const Share<T>& sh, float* orow,
+                                            F f) {
+  constexpr int E = Share<T>::E;
+  const int64_t base = sh.first(sh.v0);
+  if (sh.n > 0 && sh.inner(sh.v0) && sh.inner(sh.v0 + sh.n - 1) &&
+      (reinterpret_cast<uintptr_t>(orow + base) & (4 * E - 1)) == 0) {
+    for (int i = threadIdx.x; i < sh.n; i += kFThreads) {
+      float x[E];
+      Raw<T>::unpack(sh.buf[i], x);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 p = f(make_float2(x[e], x[e + 1]));
+        x[e] = p.x;
+        x[e + 1] = p.y;
+      }
+      float* o = orow + base + static_cast<int64_t>(i) * E;
+      if constexpr (E == 8)
+        store_8(o, x);
+      else
+        *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+    return;
+  }
+  const int64_t i0 = max(int64_t{0}, base);
+  const int64_t i1 = min(sh.v, sh.first(sh.v0 + sh.n));
+  const T* share = reinterpret_cast<const T*>(sh.buf) - base;
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += kFThreads) {
+    const float x = to_f32(share[i]);
+    orow[i] = f(make_float2(x, x)).x;
+  }
+}
+
+// One-hot and empty rows.
+template <class T>
+__device__ __forceinline__ void write_one_hot(const Share<T>& sh, float* orow,
+                                              int64_t arg) {
+  const int64_t i0 = max(int64_t{0}, sh.first(sh.v0));
+  const int64_t i1 = min(sh.v, sh.first(sh.v0 + sh.n));
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += kFThreads)
+    orow[i] = i == arg ? 1.0f : 0.0f;
+}
+
+// Kept values' probabilities (kAll: every value is kept).
+template <class T, bool kAll>
+__device__ __forceinline__ void write_kept(const Share<T>& sh, float* orow,
+                                           float m, float low, double z,
+                                           float t) {
+  const float inv_z = static_cast<float>(1.0 / z);
+  const FineScale f = fine_scale_of(t);
+  if (m == CUDART_INF_F || t == CUDART_INF_F) {
+    write_share(sh, orow, [&](float2 x) {
+      return make_float2(x.x >= low ? weight32(x.x, m, f.hi) * inv_z : 0.0f,
+                         x.y >= low ? weight32(x.y, m, f.hi) * inv_z : 0.0f);
+    });
+    return;
+  }
+  write_share(sh, orow, [&](float2 x) {
+    float2 p = mul2(fine_weight2(x, m, f), make_float2(inv_z, inv_z));
+    if (kAll) return make_float2(fmaxf(p.x, 0.0f), fmaxf(p.y, 0.0f));  // NaN
+    return make_float2(x.x >= low ? p.x : 0.0f, x.y >= low ? p.y : 0.0f);
+  });
+}
+
+// Probabilities with top-k or top-p for some rows at least.
+template <class T>
+__global__ void __launch_bounds__(kFThreads, kKeptBlocks) kept_rows_kernel(RowArgs a) {
   const auto cl = cooperative_groups::this_cluster();
   __shared__ RowShared rs;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  uint4* buf = row_smem;
-  FilterShared* fs = nullptr;
-  if (kFilter) {
-    fs = reinterpret_cast<FilterShared*>(row_smem);
-    buf += (sizeof(FilterShared) + 15) / 16;
-  }
+  FilterShared* fs = reinterpret_cast<FilterShared*>(row_smem);
+  uint4* buf = row_smem + (sizeof(FilterShared) + 15) / 16;
   fill_exp_table(rs.tab);
   __syncthreads();
-  const int cs = static_cast<int>(cl.num_blocks());
-  const int64_t rows = static_cast<int64_t>(a.rows.batch) * a.rows.positions;
-  const int64_t step = gridDim.x / cs;
-  for (int64_t r = blockIdx.x / cs; r < rows; r += step) {
-    cl.sync();  // the last row's slots are free (and every block runs)
-    const int b = static_cast<int>(r / a.rows.positions);
-    const int j = static_cast<int>(r % a.rows.positions);
-    const Setting set = setting_of(a.set, b);
-    Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
-    const Kept kept = keep_row<T, kFilter>(cl, sh, buf, set, rs, fs);
-    float* orow = a.out + r * a.rows.vocab;
-    const int64_t i0 = max(int64_t{0}, sh.first(sh.v0));
-    const int64_t i1 = min(sh.v, sh.first(sh.v0 + sh.n));
-    const T* share = reinterpret_cast<const T*>(buf) - sh.first(sh.v0);
-    if (kept.arg < 0 || !(set.t > 0.0f)) {
-      for (int64_t i = i0 + threadIdx.x; i < i1; i += kFThreads)
-        orow[i] = i == kept.arg && kept.z > 0.0 ? 1.0f : 0.0f;
-    } else {
-      const float inv_z = static_cast<float>(1.0 / kept.z);
-      for (int64_t i = i0 + threadIdx.x; i < i1; i += kFThreads) {
-        const float x = to_f32(share[i]);
-        orow[i] = x >= kept.low ? weight32(x, kept.m, sh.scale) * inv_z : 0.0f;
-      }
-    }
-  }
+  cl.sync();  // every block runs before any writes into another
+  const int64_t r = blockIdx.x / cl.num_blocks();
+  const int b = static_cast<int>(r / a.rows.positions);
+  const int j = static_cast<int>(r % a.rows.positions);
+  const Setting set = setting_of(a.set, b);
+  Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
+  const Kept kept = keep_row(cl, sh, buf, set, rs, *fs);
+  float* orow = a.out + r * a.rows.vocab;
+  if (kept.arg < 0 || !(set.t > 0.0f))
+    write_one_hot(sh, orow, kept.arg);
+  else
+    write_kept<T, false>(sh, orow, kept.m, kept.low, kept.z, set.t);
   cl.sync();  // no block leaves while another may still write into it
+}
+
+// Plain softmax rows: the largest value and the sum in the pass that loads
+// the row into shared memory (a running maximum a warp), one exchange over
+// the cluster, and the pass that writes. Memory bounds it.
+struct SoftShared {
+  SpanSum part[kFWarps];
+  uint32_t top;
+  SpanSum slot[kMaxCluster];  // the cluster's blocks
+};
+
+template <class T>
+__global__ void __launch_bounds__(kFThreads, kSoftBlocks)
+    soft_rows_kernel(RowArgs a) {
+  constexpr int U = 4;
+  const auto cl = cooperative_groups::this_cluster();
+  __shared__ SoftShared ss;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int rank = static_cast<int>(cl.block_rank());
+  const int tid = static_cast<int>(threadIdx.x);
+  if (tid == 0) ss.top = 0;
+  cl.sync();  // every block runs before any writes into another
+  const int64_t r = blockIdx.x / cs;
+  const int b = static_cast<int>(r / a.rows.positions);
+  const int j = static_cast<int>(r % a.rows.positions);
+  const float t = setting_of(a.set, b).t;
+  const bool greedy = !(t > 0.0f);
+  Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
+  const Span sp = span_of(sh.nv, rank, cs);
+  sh.buf = row_smem;
+  sh.v0 = sp.v0;
+  sh.n = sp.v1 - sp.v0;
+  const FineScale f = greedy ? FineScale{0.0f, 0.0f} : fine_scale_of(t);
+  LaneStat st{-CUDART_INF_F, 0.0, INT32_MAX};
+  for (int i0 = 0; i0 < sh.n; i0 += U * kFThreads) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      raw[u] = load_vec(sh, sp.v0 + i0 + u * kFThreads + tid, sp.v1);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * kFThreads + tid < sh.n)
+        row_smem[i0 + u * kFThreads + tid] = raw[u];
+    auto index = [&](int u) {
+      return sh.first(sp.v0 + i0 + u * kFThreads + tid);
+    };
+    if (greedy)
+      take_vecs<T, true, kNoSum>(raw, index, f, &ss.top, st);
+    else
+      take_vecs<T, false, kFineSum>(raw, index, f, &ss.top, st);
+  }
+  st.s = warp_sum64(st.s);
+  if (lane_id() == 0) ss.part[warp_id()] = SpanSum{st.s, st.m, st.arg};
+  __syncthreads();
+  if (warp_id() == 0) {
+    const SpanSum p = join_sums(ss.part, kFWarps, t);
+    if (lane_id() < cs) *cl.map_shared_rank(&ss.slot[rank], lane_id()) = p;
+  }
+  cl.sync();
+  const SpanSum row = join_sums(ss.slot, cs, t);
+  float* orow = a.out + r * a.rows.vocab;
+  if (greedy || !(row.m > -CUDART_INF_F))
+    write_one_hot(sh, orow, row.m > -CUDART_INF_F ? row.arg : -1);
+  else
+    write_kept<T, true>(sh, orow, row.m, -CUDART_INF_F, row.s, t);
 }
 
 // The next row that may be needed, found by the first block's first warp:
@@ -669,7 +794,7 @@ __device__ __forceinline__ int64_t next_row(const RowArgs& a, RowQueue& q) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(kFThreads) stat_rows_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kFThreads, kKeptBlocks) stat_rows_kernel(RowArgs a) {
   const auto cl = cooperative_groups::this_cluster();
   __shared__ RowShared rs;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -697,7 +822,7 @@ __global__ void __launch_bounds__(kFThreads) stat_rows_kernel(RowArgs a) {
     const Setting set = setting_of(a.set, b);
     const T* row = row_ptr<T>(a.rows, b, j);
     Share<T> sh(row, a.rows.vocab);
-    const Kept kept = keep_row<T, true>(cl, sh, buf, set, rs, fs);
+    const Kept kept = keep_row(cl, sh, buf, set, rs, *fs);
     if (leader && threadIdx.x == 0) {
       RowStat st;
       st.z = kept.z;
@@ -744,7 +869,7 @@ static int row_cluster(const sg_rows& r) {
 
 template <class Kernel>
 static int launch_rows(Kernel* kernel, const RowArgs& a, bool filter,
-                       int* cache, cudaStream_t st) {
+                       int64_t most, int* cache, cudaStream_t st) {
   const int cs = row_cluster(a.rows);
   const int elems = a.rows.dtype == SG_F32 ? 4 : 8;
   const int64_t vecs = ceil_div(ceil_div(a.rows.vocab + elems - 1, elems), cs);
@@ -756,27 +881,26 @@ static int launch_rows(Kernel* kernel, const RowArgs& a, bool filter,
       ensure_dyn_smem(kernel, static_cast<size_t>(bytes) + 1024, cache);
   if (rc != SG_OK) return rc;
   const int64_t rows = static_cast<int64_t>(a.rows.batch) * a.rows.positions;
-  const int64_t static_bytes = sizeof(RowShared) + 1024;
-  const int per_sm = static_cast<int>(std::min<int64_t>(
-      2048 / kFThreads, (227 * 1024) / (bytes + static_bytes)));
-  const int64_t clusters = std::max<int64_t>(1, 148 * per_sm / cs);
-  return launch_after(kernel,
-                      static_cast<unsigned>(std::min(rows, clusters) * cs),
-                      kFThreads, cs, a, st, static_cast<size_t>(bytes));
+  if (rows > INT32_MAX / kMaxCluster) return SG_ERR_UNSUPPORTED;
+  const int64_t clusters = std::min(rows, most / cs);
+  return launch_after(kernel, static_cast<unsigned>(clusters * cs), kFThreads,
+                      cs, a, st, static_cast<size_t>(bytes));
 }
 
 template <class T>
 static int write_rows(const RowArgs& a, bool filter, cudaStream_t st) {
   static int cache[2][64];
-  return filter
-      ? launch_rows(write_rows_kernel<T, true>, a, true, cache[1], st)
-      : launch_rows(write_rows_kernel<T, false>, a, false, cache[0], st);
+  return filter ? launch_rows(kept_rows_kernel<T>, a, true, INT32_MAX,
+                              cache[1], st)
+                : launch_rows(soft_rows_kernel<T>, a, false, INT32_MAX,
+                              cache[0], st);
 }
 
 template <class T>
 static int stat_rows(const RowArgs& a, cudaStream_t st) {
   static int cache[64];
-  return launch_rows(stat_rows_kernel<T>, a, true, cache, st);
+  return launch_rows(stat_rows_kernel<T>, a, true, kKeptBlocks * 148, cache,
+                     st);
 }
 
 int launch_row_stats(const sg_rows& rows, const sg_sampling& set,

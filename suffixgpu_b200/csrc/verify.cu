@@ -62,86 +62,6 @@ struct VerifyArgs {
   int32_t* marked;    // and which
 };
 
-// What a lane knows of its warp's span so far.
-struct LaneStat {
-  float m;      // the warp's largest value
-  double s;     // this lane's sum, relative to m
-  int32_t arg;  // lowest index of the largest value
-};
-
-// Takes U vectors a lane into `st`; index(u) is the row index of vector u's
-// first element. kArg: the lowest index of the largest value, looked for
-// where the vectors reach the block's largest so far (s_top); kSum: the
-// weights.
-template <class T, bool kArg, bool kSum, int U, class Index>
-__device__ __forceinline__ void take_vecs(const uint4 (&raw)[U], Index index,
-                                          float scale, uint32_t* s_top,
-                                          LaneStat& st) {
-  constexpr int E = RowVecs<T>::E;
-  const float tm = warp_max(canon(Raw<T>::vec_max(raw)));
-  bool up = kArg ? tm >= st.m && tm > -CUDART_INF_F : tm > st.m;
-  if (kArg && up) {
-    uint32_t old = 0;
-    if (lane_id() == 0) old = atomicMax(s_top, order_key(tm));
-    up = order_key(tm) >= __shfl_sync(SG_FULL_MASK, old, 0);
-  }
-  if (up) {
-    if (kSum && st.s != 0.0) st.s *= weight32(st.m, tm, scale);
-    if (kArg) {
-      int32_t at = tm == st.m ? st.arg : INT32_MAX;
-#pragma unroll
-      for (int u = U - 1; u >= 0; --u) {
-        float x[E];
-        Raw<T>::unpack(raw[u], x);
-        const int32_t i0 = static_cast<int32_t>(index(u));
-#pragma unroll
-        for (int e = E - 1; e >= 0; --e)
-          if (x[e] == tm) at = min(at, i0 + e);
-      }
-      st.arg = __reduce_min_sync(SG_FULL_MASK, at);
-    }
-    st.m = tm;
-  }
-  if (kSum && st.m > -CUDART_INF_F) {
-    const float2 nm = make_float2(-st.m, -st.m);
-    const float2 sc = make_float2(scale, scale);
-    float2 acc = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[E];
-      Raw<T>::unpack(raw[u], x);
-      float2 p[E / 2];
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        p[e] = mul2(add2(make_float2(x[2 * e], x[2 * e + 1]), nm), sc);
-        p[e] = make_float2(exp2_fast(p[e].x), exp2_fast(p[e].y));
-      }
-#pragma unroll
-      for (int w = E / 4; w > 0; w /= 2)
-#pragma unroll
-        for (int e = 0; e < w; ++e) p[e] = add2(p[e], p[e + w]);
-      acc = add2(acc, p[0]);
-    }
-    float ts = acc.x + acc.y;
-    // NaN: masked NaN logits, +inf, or an infinite temperature's scale of 0
-    // on -inf; such vectors are summed again with each case told apart
-    if (ts != ts) {
-      ts = 0.0f;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[E];
-        Raw<T>::unpack(raw[u], x);
-        float us = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          us += weight32(canon(x[e]), st.m, scale);
-        ts += us;
-      }
-    }
-    st.s += ts;
-  }
-}
-
 // One warp's span of a row. The row's partial vectors at its two ends are
 // loaded first and taken last, so that they cost no latency of their own.
 template <class T, bool kArg, bool kSum>
@@ -164,13 +84,14 @@ __device__ __forceinline__ Part warp_stats(const RowVecs<T>& rv, Span sp,
       const int v = t0 + u * 32 + lane_id();
       if (v < sp.v1 && rv.inner(v)) raw[u] = load_16(rv.row + rv.first(v));
     }
-    take_vecs<T, kArg, kSum>(
-        raw, [&](int u) { return rv.first(t0 + u * 32 + lane_id()); }, scale,
-        s_top, st);
+    take_vecs<T, kArg, kSum ? kFastSum : kNoSum>(
+        raw, [&](int u) { return rv.first(t0 + u * 32 + lane_id()); },
+        FineScale{scale, 0.0f}, s_top, st);
   }
   if (edges)
-    take_vecs<T, kArg, kSum>(
-        edge, [&](int) { return rv.first(ev); }, scale, s_top, st);
+    take_vecs<T, kArg, kSum ? kFastSum : kNoSum>(
+        edge, [&](int) { return rv.first(ev); },
+        FineScale{scale, 0.0f}, s_top, st);
   float s = 0.0f;
   if (kSum) {
     s = static_cast<float>(st.s);

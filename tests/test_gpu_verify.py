@@ -281,8 +281,11 @@ def test_strides_and_alignment(dtype):
             assert torch.equal(got[1], want[1])
         pr = ops.target_probs(view[:, :k + 1], 0.9, top_p=0.8)
         assert torch.equal(pr, ops.target_probs(logits, 0.9, top_p=0.8))
+        # a row's sum is taken in groups that follow its alignment, so two
+        # alignments agree to rounding: each is within the bound that
+        # _probs_close derives, and so within twice that of the other
         pr = ops.target_probs(view[:, :k + 1], 0.9)
-        assert torch.equal(pr, ops.target_probs(logits, 0.9))
+        _probs_close(pr, logits, [0.9] * b, [0] * b, [1.0] * b)
     same = logits[:1, :1].expand(b, k + 1, v)
     _sampled(same, draft, u, nv)
     odd = torch.empty(v * 4 + 7, dtype=dtype, device=DEV)
