@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
+#include <cmath>
+
 #include "sg_common.cuh"
 
 namespace sg {
@@ -528,6 +530,21 @@ __device__ __forceinline__ SpanSum join_sums(const SpanSum* parts, int n,
   p.s = warp_sum64(s);
   p.m = m;
   return p;
+}
+
+// A weight's relative error is 3 * 2^-24 * ln2 = 1.24e-7 times its depth z
+// (its exponent of 2) plus 2^-22: at most kDeepGuard for one weight, whose
+// depth ends at 126. In a row's sum it counts by weight, and the weights'
+// mean depth is at most log2(V): it is their entropy less log2 of their sum,
+// and the largest weight is 1. Further errors: 2^-22 for each time the
+// largest value grew (at most once a tile) or spans were joined (2), and
+// 2^-24 for each of the at most 20 fp32 operations on a weight's way.
+constexpr double kDeepGuard = 1.7e-5;
+// `tile`: values of a row taken in at a time.
+inline double guard_of(int64_t vocab, int64_t tile) {
+  const int64_t tiles = ceil_div(vocab, tile) + 1;
+  return 1.25e-7 * std::log2(static_cast<double>(vocab) + 1.0) +
+         2.4e-7 * static_cast<double>(2 + tiles) + 1.2e-6;
 }
 
 // ---------------------------------------------------------------------------

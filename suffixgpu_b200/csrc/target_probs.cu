@@ -16,8 +16,10 @@ constexpr int kFThreads = 256;
 constexpr int kFWarps = kFThreads / 32;
 constexpr int kSoftBlocks = 5;  // blocks on an SM, plain softmax
 constexpr int kKeptBlocks = 3;  // and with filters
-constexpr int kBins = 2048;
-constexpr int kList = 2048;      // candidates the first block can hold
+constexpr int kBins = 1024;      // of a window; the last takes the rest
+constexpr float kPlaces = 64.0f;  // places told apart in a bin
+constexpr int kWindows = 4;      // looked at before bisect_row
+constexpr int kList = 1024;      // candidates the first block can hold
 constexpr int kOwn = kList / kFThreads;
 constexpr double kFix = 17592186044416.0;  // 2^44: unit of candidates' sums
 
@@ -30,9 +32,10 @@ struct Kept {
 };
 
 struct RowShared {
-  float m[kMaxCluster];  // slots the cluster's blocks write into each other
-  int32_t arg[kMaxCluster];
+  SpanSum part[kFWarps];
+  SpanSum slot[kMaxCluster];  // the cluster's blocks write into each other
   double s[kMaxCluster];
+  uint32_t top;
   int32_t next;
   float redf[kFWarps];
   int32_t redi[kFWarps];
@@ -41,18 +44,31 @@ struct RowShared {
   double tab[kExpTable];
 };
 
+// How the first block goes on after a window's counts.
+struct Plan {
+  int32_t off;    // >= 0: count the window of bins from here on
+  int32_t give;   // 1: bisect_row
+  int32_t bk;     // bin of the k-th value
+  int32_t above;  // values in bins before it
+  int32_t p0, p1; // bins in which top-p's border is looked for
+};
+
 struct FilterShared {
   uint32_t hist[kBins];  // this block's counts
-  uint32_t tot[kBins];   // first block: the row's
+  uint32_t offs[kBins];  // and their places in the bins, summed
   uint32_t list[kList];  // this block's candidates (order keys)
   int32_t listed;
   int32_t n[kMaxCluster];
+  uint32_t nall[kMaxCluster];
   double a[kMaxCluster];
   uint64_t redl[kFWarps];
-  // the plan: the bin of the k-th value, the values in bins before it, and
-  // the bins [p0, p1] in which top-p's border is looked for
-  int32_t bk, above, p0, p1;
-  // the result
+  Plan plan;
+  // first block, over the windows so far
+  int32_t seen;          // values in earlier windows
+  float mass;            // and their weights, about
+  int32_t k_found, pick;
+  float need;
+  // the result; done 0: bisect_row, 2: sum the row exactly and come again
   double z;
   float low;
   int32_t done;
@@ -109,21 +125,33 @@ struct Share : RowVecs<T> {
       : RowVecs<T>(row, vocab) {}
 
   // Bins of equal width down from the largest value, rounded to nearest;
-  // the last takes everything beyond, NaN and -inf too. Monotone in x.
+  // NaN and -inf come last. Monotone in x.
   __device__ __forceinline__ int bin(float x) const {
-    const float t = fminf((m - x) * bin_scale, kBins - 1.0f);
-    return __float_as_uint(t + 8388608.0f) & (kBins - 1);
+    const float t = fminf((m - x) * bin_scale, 4194303.0f);
+    return __float_as_uint(t + 8388608.0f) & 0x7fffff;
+  }
+  // Where in its bin a value lies, from 0 to kPlaces.
+  __device__ __forceinline__ uint32_t place(float x, int b) const {
+    const float t = (m - x) * bin_scale - (static_cast<float>(b) - 0.5f);
+    return static_cast<uint32_t>(fmaxf(t, 0.0f) * kPlaces + 0.5f);
   }
   __device__ __forceinline__ double weight(float x) const {
     return weight64(x, m64, scale64, tab);
   }
   // f(value, row index) for this thread's values; the vectors' order is the
-  // same in every pass. Values outside the row are left out.
+  // same in every pass. Values outside the row are left out. With kTop,
+  // vectors without a value >= from are passed over.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
+    each_from<false>(0.0f, f);
+  }
+  template <bool kTop, class F>
+  __device__ __forceinline__ void each_from(float from, F f) const {
     for (int i = threadIdx.x; i < n; i += kFThreads) {
+      const uint4 raw[1] = {buf[i]};
+      if (kTop && !(Raw<T>::vec_max(raw) >= from)) continue;
       float x[E];
-      Raw<T>::unpack(buf[i], x);
+      Raw<T>::unpack(raw[0], x);
       const int64_t at = this->first(v0 + i);
       if (this->inner(v0 + i)) {
 #pragma unroll
@@ -183,14 +211,14 @@ __device__ void bisect_row(const cooperative_groups::cluster_group& cl,
   if (static_cast<int>(threadIdx.x) < cs) {
     *cl.map_shared_rank(&fs.n[rank], static_cast<int>(threadIdx.x)) =
         static_cast<int32_t>(any);
-    *cl.map_shared_rank(&rs.arg[rank], static_cast<int>(threadIdx.x)) =
-        static_cast<int32_t>(not_all);
+    *cl.map_shared_rank(&fs.nall[rank], static_cast<int>(threadIdx.x)) =
+        not_all;
   }
   cl.sync();
   any = not_all = 0;
   for (int i = 0; i < cs; ++i) {
     any |= static_cast<uint32_t>(fs.n[i]);
-    not_all |= static_cast<uint32_t>(rs.arg[i]);
+    not_all |= fs.nall[i];
   }
   cl.sync();
   const uint32_t differ = any & not_all;
@@ -224,149 +252,218 @@ __device__ void bisect_row(const cooperative_groups::cluster_group& cl,
   __syncthreads();
 }
 
+// First block: reads the plan off a window's counts (all its threads).
+__device__ __forceinline__ void plan_window(
+    const cooperative_groups::cluster_group& cl, int32_t off, int32_t k,
+    float p, float octaves, float row_sum, RowShared& rs, FilterShared& fs,
+    Plan& plan) {
+  constexpr int kPer = kBins / kFThreads;
+  static_assert(kPer == 4, "a thread reads its bins as one vector");
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int tid = static_cast<int>(threadIdx.x);
+  int32_t c[kPer] = {0, 0, 0, 0};
+  float o[kPer] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int r = 0; r < cs; ++r) {
+    const FilterShared* from = cl.map_shared_rank(&fs, r);
+    const uint4 h = reinterpret_cast<const uint4*>(from->hist)[tid];
+    const uint4 f = reinterpret_cast<const uint4*>(from->offs)[tid];
+    c[0] += h.x;
+    c[1] += h.y;
+    c[2] += h.z;
+    c[3] += h.w;
+    o[0] += f.x;
+    o[1] += f.y;
+    o[2] += f.z;
+    o[3] += f.w;
+  }
+  float w[kPer];  // the weight at the mean place of a bin's values
+  int32_t cnt = 0;
+  float mass = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float at = static_cast<float>(off + tid * kPer + i) - 0.5f +
+                     o[i] / (kPlaces * fmaxf(1.0f, static_cast<float>(c[i])));
+    w[i] = exp2_fast(-at * octaves);
+    cnt += c[i];
+    mass += static_cast<float>(c[i]) * w[i];
+  }
+  const int32_t ci = warp_incl_scan(cnt);
+  float mi = mass;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float t = __shfl_up_sync(SG_FULL_MASK, mi, o);
+    if (lane_id() >= o) mi += t;
+  }
+  if (lane_id() == 31) {
+    rs.redi[warp_id()] = ci;
+    rs.redf[warp_id()] = mi;
+  }
+  if (tid == 0) {
+    fs.pick = INT32_MAX;
+    if (off == 0 && !fs.k_found) {
+      fs.seen = 0;
+      fs.mass = 0.0f;
+    }
+  }
+  __syncthreads();
+  const int32_t seen = fs.seen;
+  const float mass_seen = fs.mass;
+  int32_t run = seen + ci - cnt;
+  float mr = mass_seen + (mi - mass);
+  int32_t all_c = seen;
+  float all_m = mass_seen;
+#pragma unroll
+  for (int i = 0; i < kFWarps; ++i) {
+    if (i < warp_id()) {
+      run += rs.redi[i];
+      mr += rs.redf[i];
+    }
+    all_c += rs.redi[i];
+    all_m += rs.redf[i];
+  }
+  if (k > 0 && !fs.k_found) {
+    int32_t r = run;
+    float q = mr;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (r < k && k <= r + c[i]) {
+        plan.bk = off + tid * kPer + i;
+        plan.above = r;
+        fs.pick = plan.bk;
+        fs.need = p * (q + static_cast<float>(k - r) * w[i]);
+      }
+      r += c[i];
+      q += static_cast<float>(c[i]) * w[i];
+    }
+  }
+  if (k <= 0 && tid == 0) fs.need = p * row_sum;
+  __syncthreads();
+  bool k_now = false;
+  if (k > 0 && !fs.k_found) {
+    k_now = fs.pick != INT32_MAX;
+    __syncthreads();
+    if (tid == 0) {
+      fs.pick = INT32_MAX;
+      if (k_now) fs.k_found = 1;
+    }
+    __syncthreads();
+  }
+  // the border of top-p, once the kept mass is known
+  int32_t next = -1;
+  if (p < 1.0f && (k <= 0 || fs.k_found)) {
+    if (k_now && off > 0) {
+      next = 0;  // it may lie in an earlier window
+    } else {
+      float q = mr;
+      int32_t at = INT32_MAX;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        q += static_cast<float>(c[i]) * w[i];
+        if (q >= fs.need && tid * kPer + i < kBins - 1)
+          at = min(at, off + tid * kPer + i);
+      }
+      if (at != INT32_MAX) atomicMin(&fs.pick, at);
+      __syncthreads();
+      at = fs.pick;
+      // the border does not lie beyond the k-th value
+      if (k > 0 && plan.bk < off + kBins - 1) at = min(at, plan.bk);
+      if (at == INT32_MAX) {
+        next = off + kBins - 1;
+      } else if (tid == 0) {
+        plan.p0 = max(at - 1, 0);
+        plan.p1 = k > 0 ? min(at + 1, plan.bk) : at + 1;
+      }
+    }
+  } else if (k > 0 && !fs.k_found) {
+    next = off + kBins - 1;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    plan.off = next;
+    plan.give = next >= kWindows * (kBins - 1);
+    fs.seen = next == 0 ? 0 : all_c;
+    fs.mass = next == 0 ? 0.0f : all_m;
+  }
+  __syncthreads();
+}
+
 // The smallest kept value and the kept mass of a row with top-k (k > 0) or
 // top-p (0 < p < 1) or both; left in fs.low and fs.z of every block.
 //
-// One pass counts the values in bins; the first block finds the bin of the
-// k-th value from the counts, and from counts times the bins' middle weights
-// the bin top-p's border should lie in. A second pass sums the weights
+// One pass counts the values in bins from the largest down, a window of bins
+// at a time (mostly one is enough); the first block finds the bin of the
+// k-th value from the counts, and from counts and mean places in the bins
+// (off by about 1e-5) the bin top-p's border should lie in. A second pass sums the weights
 // ahead of those bins in 64 bits and lists the values inside them, from
 // which the first block takes both borders exactly: top-k by counting,
 // top-p by 64-bit sums, whose order does not matter (fixed point). Whether
 // the border lies in the bins looked at shows in the exact sums; if not, or
-// if the list is too short, bisect_row finds it.
+// if the list is too short, bisect_row finds it. Without top-k, top-p's
+// share is taken of the row's fp32 sum where the border is clear of that
+// sum's error, else of its exact sum.
 template <class T>
 __device__ void filter_row(const cooperative_groups::cluster_group& cl,
-                           Share<T>& sh, int32_t k, float p, RowShared& rs,
-                           FilterShared& fs) {
+                           Share<T>& sh, int32_t k, float p, double row_sum,
+                           double guard, RowShared& rs, FilterShared& fs) {
   const int cs = static_cast<int>(cl.num_blocks());
   const int rank = static_cast<int>(cl.block_rank());
   const int tid = static_cast<int>(threadIdx.x);
   const bool with_p = p < 1.0f;
-  // 32 octaves of weight or 32 units of logits, whichever is shorter
-  const float range = fminf(32.0f / sh.scale, 32.0f);
-  sh.bin_scale = fminf((kBins - 1.0f) / range, 1e30f);
-
+  // 64 bins an octave of weight, 96 a unit of logits at least
+  sh.bin_scale = fminf(fmaxf(64.0f * sh.scale, 96.0f), 1e30f);
+  if (tid == 0) {
+    fs.listed = 0;
+    fs.k_found = 0;
+    fs.plan.bk = -1;
+  }
   // fs.hist is zero (cleared by the caller before its barrier)
-  sh.each([&](float x, int64_t) {
-    const int b = sh.bin(x);
-    if (b < kBins - 1) atomicAdd(&fs.hist[b], 1u);
-  });
-  if (tid == 0) fs.listed = 0;
-  cl.sync();
-  {  // the row's counts, a slice of bins a block, into the first block
-    const int slice = kBins / cs;
-    uint32_t* tot = cl.map_shared_rank(fs.tot, 0);
-    for (int i = rank * slice + tid; i < (rank + 1) * slice; i += kFThreads) {
-      uint32_t c = 0;
-      for (int r = 0; r < cs; ++r) c += cl.map_shared_rank(fs.hist, r)[i];
-      tot[i] = c;
-    }
-  }
-  cl.sync();
-  if (rank == 0) {
-    constexpr int kPer = kBins / kFThreads;
-    const float octaves = sh.scale / sh.bin_scale;  // a bin's
-    int32_t c[kPer];
-    float w[kPer];
-    int32_t cnt = 0;
-    float mass = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int b = tid * kPer + i;
-      c[i] = static_cast<int32_t>(fs.tot[b]);
-      w[i] = exp2_fast(-static_cast<float>(b) * octaves);
-      cnt += c[i];
-      mass += static_cast<float>(c[i]) * w[i];
-    }
-    int32_t ci = warp_incl_scan(cnt);
-    float mi = mass;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float t = __shfl_up_sync(SG_FULL_MASK, mi, o);
-      if (lane_id() >= o) mi += t;
-    }
-    if (lane_id() == 31) {
-      rs.redi[warp_id()] = ci;
-      rs.redf[warp_id()] = mi;
-    }
-    if (tid == 0) {
-      fs.bk = kBins;  // top-k off: every bin lies ahead of it
-      fs.above = 0;
-      fs.p0 = kBins;
-      rs.red[0] = 0.0;
-    }
-    __syncthreads();
-    int32_t c0 = ci - cnt;
-    float m0 = mi - mass;
-    float all = 0.0f;
-    for (int i = 0; i < kFWarps; ++i) {
-      if (i < warp_id()) {
-        c0 += rs.redi[i];
-        m0 += rs.redf[i];
+  for (int32_t off = 0;;) {
+    const float from = sh.m - (off + kBins) / sh.bin_scale;
+    sh.template each_from<true>(from, [&](float x, int64_t) {
+      const int b = sh.bin(x) - off;
+      if (b >= 0 && b < kBins - 1) {
+        atomicAdd(&fs.hist[b], 1u);
+        if (with_p) atomicAdd(&fs.offs[b], sh.place(x, b + off));
       }
-      all += rs.redf[i];
-    }
-    if (k > 0) {
-      int32_t run = c0;
-      float mr = m0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int b = tid * kPer + i;
-        const bool last = b == kBins - 1;
-        if (run < k && (k <= run + c[i] || last)) {
-          fs.bk = b;
-          fs.above = run;
-          rs.red[0] = mr + static_cast<float>(k - run) * w[i];
-        }
-        run += c[i];
-        mr += static_cast<float>(c[i]) * w[i];
-      }
+    });
+    cl.sync();
+    if (rank == 0) {
+      plan_window(cl, off, k, p, sh.scale / sh.bin_scale,
+                  static_cast<float>(row_sum), rs, fs, fs.plan);
+      const Plan plan = fs.plan;
       __syncthreads();
-      all = static_cast<float>(rs.red[0]);
+      if (tid > 0 && tid < cs) cl.map_shared_rank(&fs, tid)->plan = plan;
     }
-    if (with_p) {
-      const float need = p * all;
-      float incl = m0;
-      int at = kBins;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        incl += static_cast<float>(c[i]) * w[i];
-        if (incl >= need) at = min(at, tid * kPer + i);
-      }
-      if (at < kBins) atomicMin(&fs.p0, at);
-      __syncthreads();
-    }
-    const int bk = fs.bk;
-    const int mid = min(min(fs.p0, kBins - 1), bk);
-    const int above = fs.above;
+    cl.sync();
+    off = fs.plan.off;
+    if (off < 0 || fs.plan.give) break;
+    for (int i = tid; i < kBins; i += kFThreads) fs.hist[i] = fs.offs[i] = 0;
     __syncthreads();
-    if (tid < cs) {
-      FilterShared* o = cl.map_shared_rank(&fs, tid);
-      o->bk = bk;
-      o->above = above;
-      o->p0 = with_p ? max(mid - 1, 0) : kBins;
-      o->p1 = with_p ? min(mid + 1, min(bk, kBins - 1)) : -1;
-    }
   }
-  cl.sync();
+  if (fs.plan.give) {
+    bisect_row(cl, sh, k, p, rs, fs);
+    return;
+  }
 
   // exact sums ahead of the bins looked at, and the values inside them
-  const int bk = fs.bk, p0 = fs.p0, p1 = fs.p1;
+  const int bk = k > 0 ? fs.plan.bk : -1;
+  const int p0 = with_p ? fs.plan.p0 : INT32_MAX;
+  const int p1 = with_p ? fs.plan.p1 : -1;
   double s = 0.0, a = 0.0;
-  sh.each([&](float x, int64_t) {
-    const int b = sh.bin(x);
-    if (b < bk) {
-      const double w = sh.weight(x);
-      s += w;
-      if (b < p0) a += w;
-    }
-    if (b == bk || (b >= p0 && b <= p1)) {
-      const int at = atomicAdd(&fs.listed, 1);
-      if (at < kList) fs.list[at] = order_key(canon(x));
-    }
-  });
-  s = block_sum64(s, rs.red);
+  sh.template each_from<true>(
+      sh.m - (max(bk, p1) + 1) / sh.bin_scale, [&](float x, int64_t) {
+        const int b = sh.bin(x);
+        if (b < bk || (with_p && b < p0)) {
+          const double w = sh.weight(x);
+          if (b < bk) s += w;
+          if (b < p0) a += w;
+        }
+        if (b == bk || (b >= p0 && b <= p1)) {
+          const int at = atomicAdd(&fs.listed, 1);
+          if (at < kList) fs.list[at] = order_key(canon(x));
+        }
+      });
+  if (k > 0) s = block_sum64(s, rs.red);
   if (with_p) a = block_sum64(a, rs.red);
   __syncthreads();
   if (tid == 0) {
@@ -375,110 +472,170 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
     *cl.map_shared_rank(&fs.n[rank], 0) = fs.listed;
   }
   cl.sync();
-  if (rank == 0) {
-    int n = 0;
-    bool fits = true;
-    s = a = 0.0;
-    for (int r = 0; r < cs; ++r) {
-      n += fs.n[r];
-      fits = fits && fs.n[r] <= kList;
-      s += rs.s[r];
-      a += fs.a[r];
-    }
-    bool done = fits && n <= kList;
-    float low = -CUDART_INF_F;
-    double z = s;
-    if (done) {
-      // this thread's candidates: their keys, bins and fixed-point weights
-      uint32_t key[kOwn];
-      uint64_t w[kOwn];
-      bool in_k[kOwn], in_p[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        int at = tid + i * kFThreads;
-        key[i] = 0;
-        w[i] = 0;
-        in_k[i] = in_p[i] = false;
-        if (at < n) {
-          int r = 0;
-          while (at >= fs.n[r]) at -= fs.n[r++];
-          key[i] = cl.map_shared_rank(fs.list, r)[at];
-          const float x = key_value(key[i]);
-          const int b = sh.bin(x);
-          in_k[i] = b == bk;
-          in_p[i] = b >= p0 && b <= p1;
-          w[i] = static_cast<uint64_t>(
-              __double2ll_rn(sh.weight(x) * kFix));
-        }
+  for (bool exact = k > 0;; exact = true) {
+    if (rank == 0) {
+      int n = 0;
+      bool fits = true;
+      double kept = 0.0;  // values before bin bk, or the row's sum
+      a = 0.0;
+      for (int r = 0; r < cs; ++r) {
+        n += fs.n[r];
+        fits = fits && fs.n[r] <= kList;
+        kept += rs.s[r];
+        a += fs.a[r];
       }
-      // keys' differing bits among a set; the greatest key that `enough`
-      // accepts, and the set's smallest key where none but it does
-      auto border = [&](const bool (&in)[kOwn], auto enough) {
-        uint32_t any = 0, not_all = 0, least = 0xffffffffu;
+      if (!exact) kept = row_sum;
+      int done = fits && n <= kList;
+      float low = -CUDART_INF_F;
+      if (done) {
+        // this thread's candidates: their keys, bins and fixed-point weights
+        uint32_t key[kOwn];
+        uint64_t w[kOwn];
+        bool in_k[kOwn], in_p[kOwn];
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-          if (in[i]) {
-            any |= key[i];
-            not_all |= ~key[i];
-            least = min(least, key[i]);
+          int at = tid + i * kFThreads;
+          key[i] = 0;
+          w[i] = 0;
+          in_k[i] = in_p[i] = false;
+          if (at < n) {
+            int r = 0;
+            while (at >= fs.n[r]) at -= fs.n[r++];
+            key[i] = cl.map_shared_rank(fs.list, r)[at];
+            const float x = key_value(key[i]);
+            const int b = sh.bin(x);
+            in_k[i] = b == bk;
+            in_p[i] = b >= p0 && b <= p1;
+            w[i] = static_cast<uint64_t>(
+                __double2ll_rn(sh.weight(x) * kFix));
           }
         }
-        any = block_or(any, rs.redu);
-        not_all = block_or(not_all, rs.redu);
-        least = ~block_max_u32(~least, rs.redu);
-        uint32_t t = any & ~not_all;
-        for (uint32_t bits = any & not_all; bits;) {
-          const uint32_t bit = 0x80000000u >> __clz(bits);
-          bits &= ~bit;
-          if (enough(t | bit)) t |= bit;
-        }
-        return max(t, least);
-      };
-      uint32_t tk = 0;
-      if (k > 0) {
-        const int32_t want = k - fs.above;
-        tk = border(in_k, [&](uint32_t from) {
-          int32_t c = 0;
+        // The greatest key of a set that `enough` accepts (its smallest, if
+        // none but that): bit by bit over the bits in which its keys differ.
+        auto border = [&](const bool (&in)[kOwn], auto enough) {
+          uint32_t any = 0, not_all = 0, least = 0xffffffffu;
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i) c += in_k[i] && key[i] >= from;
-          return block_sum_i32(c, rs.redi) >= want;
-        });
-        uint64_t f = 0;
+          for (int i = 0; i < kOwn; ++i) {
+            if (in[i]) {
+              any |= key[i];
+              not_all |= ~key[i];
+              least = min(least, key[i]);
+            }
+          }
+          any = block_or(any, rs.redu);
+          not_all = block_or(not_all, rs.redu);
+          least = ~block_max_u32(~least, rs.redu);
+          uint32_t t = any & ~not_all;
+          for (uint32_t bits = any & not_all; bits;) {
+            const uint32_t bit = 0x80000000u >> __clz(bits);
+            bits &= ~bit;
+            if (enough(t | bit)) t |= bit;
+          }
+          return max(t, least);
+        };
+        if (k > 0) {
+          const int32_t want = k - fs.plan.above;
+          const uint32_t tk = border(in_k, [&](uint32_t from) {
+            int32_t c = 0;
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-          f += in_k[i] && key[i] >= tk ? w[i] : 0;
-          in_p[i] = in_p[i] && key[i] >= tk;
-        }
-        z += static_cast<double>(block_sum_u64(f, fs.redl)) / kFix;
-        low = key_value(tk);
-      }
-      if (with_p) {
-        const double need = static_cast<double>(p) * z;
-        auto mass = [&](uint32_t from) {
+            for (int i = 0; i < kOwn; ++i) c += in_k[i] && key[i] >= from;
+            return block_sum_i32(c, rs.redi) >= want;
+          });
           uint64_t f = 0;
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i)
-            f += in_p[i] && key[i] >= from ? w[i] : 0;
-          return a + static_cast<double>(block_sum_u64(f, fs.redl)) / kFix;
-        };
-        done = a < need && mass(0) >= need;
-        if (done) {
-          const uint32_t t =
-              border(in_p, [&](uint32_t from) { return mass(from) >= need; });
-          low = key_value(t);
-          z = mass(t);
+          for (int i = 0; i < kOwn; ++i) {
+            f += in_k[i] && key[i] >= tk ? w[i] : 0;
+            in_p[i] = in_p[i] && key[i] >= tk;
+          }
+          kept += static_cast<double>(block_sum_u64(f, fs.redl)) / kFix;
+          low = key_value(tk);
+        }
+        if (with_p) {
+          const double need = static_cast<double>(p) * kept;
+          const double slack = exact ? 0.0 : need * guard;
+          auto mass = [&](uint32_t from) {
+            uint64_t f = 0;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i)
+              f += in_p[i] && key[i] >= from ? w[i] : 0;
+            return a + static_cast<double>(block_sum_u64(f, fs.redl)) / kFix;
+          };
+          if (!(a < need - slack && mass(0) >= need + slack)) {
+            done = exact ? 0 : 2;
+          } else {
+            const uint32_t t = border(
+                in_p, [&](uint32_t from) { return mass(from) >= need; });
+            low = key_value(t);
+            kept = mass(t);
+            if (!exact &&
+                !(kept >= need + slack && mass(t + 1) < need - slack))
+              done = 2;
+          }
         }
       }
+      if (tid < cs) {
+        FilterShared* o = cl.map_shared_rank(&fs, tid);
+        o->low = low;
+        o->z = kept;
+        o->done = done;
+      }
     }
-    if (tid < cs) {
-      FilterShared* o = cl.map_shared_rank(&fs, tid);
-      o->low = low;
-      o->z = z;
-      o->done = done;
-    }
+    cl.sync();
+    if (fs.done != 2) break;
+    double all = 0.0;
+    sh.each([&](float x, int64_t) { all += sh.weight(x); });
+    all = block_sum64(all, rs.red);
+    if (tid == 0) *cl.map_shared_rank(&rs.s[rank], 0) = all;
+    cl.sync();
+  }
+  if (!fs.done) bisect_row(cl, sh, k, p, rs, fs);
+}
+
+// Loads a row's shares into shared memory and gives its largest value, the
+// lowest index of that (t not > 0) or the fp32 sum of its weights (t > 0):
+// a running maximum a warp, one exchange over the cluster. rs.top is 0.
+template <class T>
+__device__ __forceinline__ SpanSum
+load_row(const cooperative_groups::cluster_group& cl, Share<T>& sh, uint4* buf,
+         float t, RowShared& rs) {
+  constexpr int U = 4;
+  const int cs = static_cast<int>(cl.num_blocks());
+  const int rank = static_cast<int>(cl.block_rank());
+  const int tid = static_cast<int>(threadIdx.x);
+  const Span sp = span_of(sh.nv, rank, cs);
+  sh.buf = buf;
+  sh.v0 = sp.v0;
+  sh.n = sp.v1 - sp.v0;
+  const bool greedy = !(t > 0.0f);
+  const FineScale f = greedy ? FineScale{0.0f, 0.0f} : fine_scale_of(t);
+  LaneStat st{-CUDART_INF_F, 0.0, INT32_MAX};
+  for (int i0 = 0; i0 < sh.n; i0 += U * kFThreads) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      raw[u] = load_vec(sh, sp.v0 + i0 + u * kFThreads + tid, sp.v1);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * kFThreads + tid < sh.n)
+        buf[i0 + u * kFThreads + tid] = raw[u];
+    auto index = [&](int u) {
+      return sh.first(sp.v0 + i0 + u * kFThreads + tid);
+    };
+    if (greedy)
+      take_vecs<T, true, kNoSum>(raw, index, f, &rs.top, st);
+    else
+      take_vecs<T, false, kFineSum>(raw, index, f, &rs.top, st);
+  }
+  st.s = warp_sum64(st.s);
+  if (lane_id() == 0) rs.part[warp_id()] = SpanSum{st.s, st.m, st.arg};
+  __syncthreads();
+  if (warp_id() == 0) {
+    const SpanSum p = join_sums(rs.part, kFWarps, t);
+    if (lane_id() < cs) *cl.map_shared_rank(&rs.slot[rank], lane_id()) = p;
+    if (lane_id() == 0) rs.top = 0;
   }
   cl.sync();
-  if (!fs.done) bisect_row(cl, sh, k, p, rs, fs);
+  return join_sums(rs.slot, cs, t);
 }
 
 // ---------------------------------------------------------------------------
@@ -487,79 +644,40 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
 template <class T>
 __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
                          Share<T>& sh, uint4* buf, const Setting& set,
-                         RowShared& rs, FilterShared& fs) {
-  constexpr int U = 8;
+                         double guard, RowShared& rs, FilterShared& fs) {
   const int cs = static_cast<int>(cl.num_blocks());
   const int rank = static_cast<int>(cl.block_rank());
   const int tid = static_cast<int>(threadIdx.x);
-  const Span sp = span_of(sh.nv, rank, cs);
-  sh.buf = buf;
-  sh.v0 = sp.v0;
-  sh.n = sp.v1 - sp.v0;
-  sh.tab = rs.tab;
-  for (int i = tid; i < kBins; i += kFThreads) fs.hist[i] = 0;
-  float m = -CUDART_INF_F;
-  for (int i0 = tid; i0 < sh.n; i0 += U * kFThreads) {
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      raw[u] = load_vec(sh, sp.v0 + i0 + u * kFThreads, sp.v1);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u * kFThreads < sh.n) buf[i0 + u * kFThreads] = raw[u];
-    m = fmaxf(m, Raw<T>::vec_max(raw));
-  }
-  m = warp_max(canon(m));
-  if (lane_id() == 0) rs.redf[warp_id()] = m;
-  __syncthreads();
-  for (int i = 0; i < kFWarps; ++i) m = fmaxf(m, rs.redf[i]);
-  if (tid < cs) *cl.map_shared_rank(&rs.m[rank], tid) = m;
-  cl.sync();
-  Kept kept{0.0, -CUDART_INF_F, -CUDART_INF_F, -1};
-  for (int i = 0; i < cs; ++i) kept.m = fmaxf(kept.m, rs.m[i]);
-  if (!(kept.m > -CUDART_INF_F)) return kept;  // no mass
-  sh.m = kept.m;
-  sh.m64 = static_cast<double>(kept.m);
+  for (int i = tid; i < kBins; i += kFThreads) fs.hist[i] = fs.offs[i] = 0;
+  const SpanSum row = load_row(cl, sh, buf, set.t, rs);
+  Kept kept{0.0, row.m, -CUDART_INF_F, -1};
+  if (!(row.m > -CUDART_INF_F)) return kept;  // no mass
   kept.arg = 0;
   if (!(set.t > 0.0f)) {  // greedy: the first largest value
-    int32_t at = INT32_MAX;
-    sh.each([&](float x, int64_t i) {
-      if (x == kept.m) at = min(at, static_cast<int32_t>(i));
-    });
-    at = __reduce_min_sync(SG_FULL_MASK, at);
-    if (lane_id() == 0) rs.redi[warp_id()] = at;
-    __syncthreads();
-    for (int i = 0; i < kFWarps; ++i) at = min(at, rs.redi[i]);
-    if (tid < cs) *cl.map_shared_rank(&rs.arg[rank], tid) = at;
-    cl.sync();
-    for (int i = 0; i < cs; ++i) at = min(at, rs.arg[i]);
-    kept.arg = at;
+    kept.arg = row.arg;
     kept.z = 1.0;
     return kept;
   }
+  sh.m = row.m;
+  sh.m64 = static_cast<double>(row.m);
   sh.scale = scale_of(set.t);
   sh.scale64 = scale64_of(set.t);
+  sh.tab = rs.tab;
   const int32_t k = set.k > 0 && set.k < sh.v ? set.k : 0;
   const float p = set.p < 1.0f ? set.p : 1.0f;
-  if (kept.m == CUDART_INF_F || !(p > 0.0f)) {
+  double s = 0.0;
+  if (row.m == CUDART_INF_F || !(p > 0.0f)) {
     // only the largest value has mass, or is kept
-    int32_t c = 0;
-    sh.each([&](float x, int64_t) { c += x == kept.m; });
-    c = block_sum_i32(c, rs.redi);
-    if (tid < cs) *cl.map_shared_rank(&rs.arg[rank], tid) = c;
-    cl.sync();
-    for (int i = 0; i < cs; ++i) kept.z += rs.arg[i];
-    kept.low = kept.m;
-    return kept;
-  }
-  if (k > 0 || p < 1.0f) {
-    filter_row(cl, sh, k, p, rs, fs);
+    sh.each([&](float x, int64_t) { s += x == row.m ? 1.0 : 0.0; });
+    kept.low = row.m;
+  } else if (k > 0 || p < 1.0f) {
+    filter_row(cl, sh, k, p, row.s, guard, rs, fs);
     kept.low = fs.low;
     kept.z = fs.z;
     return kept;
+  } else {
+    sh.each([&](float x, int64_t) { s += sh.weight(x); });
   }
-  double s = 0.0;
-  sh.each([&](float x, int64_t) { s += sh.weight(x); });
   s = block_sum64(s, rs.red);
   if (tid < cs) *cl.map_shared_rank(&rs.s[rank], tid) = s;
   cl.sync();
@@ -573,7 +691,8 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
 struct RowArgs {
   sg_rows rows;
   sg_sampling set;
-  float* out;  // [B, positions, V]
+  double guard;  // relative error of a row's fp32 sum
+  float* out;    // [B, positions, V]
   // statistics for the verification
   const int32_t* draft;
   const int32_t* num_valid;
@@ -670,14 +789,14 @@ __global__ void __launch_bounds__(kFThreads, kKeptBlocks) kept_rows_kernel(RowAr
   FilterShared* fs = reinterpret_cast<FilterShared*>(row_smem);
   uint4* buf = row_smem + (sizeof(FilterShared) + 15) / 16;
   fill_exp_table(rs.tab);
-  __syncthreads();
+  if (threadIdx.x == 0) rs.top = 0;
   cl.sync();  // every block runs before any writes into another
   const int64_t r = blockIdx.x / cl.num_blocks();
   const int b = static_cast<int>(r / a.rows.positions);
   const int j = static_cast<int>(r % a.rows.positions);
   const Setting set = setting_of(a.set, b);
   Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
-  const Kept kept = keep_row(cl, sh, buf, set, rs, *fs);
+  const Kept kept = keep_row(cl, sh, buf, set, a.guard, rs, *fs);
   float* orow = a.out + r * a.rows.vocab;
   if (kept.arg < 0 || !(set.t > 0.0f))
     write_one_hot(sh, orow, kept.arg);
@@ -689,66 +808,26 @@ __global__ void __launch_bounds__(kFThreads, kKeptBlocks) kept_rows_kernel(RowAr
 // Plain softmax rows: the largest value and the sum in the pass that loads
 // the row into shared memory (a running maximum a warp), one exchange over
 // the cluster, and the pass that writes. Memory bounds it.
-struct SoftShared {
-  SpanSum part[kFWarps];
-  uint32_t top;
-  SpanSum slot[kMaxCluster];  // the cluster's blocks
-};
-
 template <class T>
 __global__ void __launch_bounds__(kFThreads, kSoftBlocks)
     soft_rows_kernel(RowArgs a) {
-  constexpr int U = 4;
   const auto cl = cooperative_groups::this_cluster();
-  __shared__ SoftShared ss;
+  __shared__ RowShared rs;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int cs = static_cast<int>(cl.num_blocks());
-  const int rank = static_cast<int>(cl.block_rank());
-  const int tid = static_cast<int>(threadIdx.x);
-  if (tid == 0) ss.top = 0;
+  if (threadIdx.x == 0) rs.top = 0;
   cl.sync();  // every block runs before any writes into another
-  const int64_t r = blockIdx.x / cs;
+  const int64_t r = blockIdx.x / cl.num_blocks();
   const int b = static_cast<int>(r / a.rows.positions);
   const int j = static_cast<int>(r % a.rows.positions);
   const float t = setting_of(a.set, b).t;
-  const bool greedy = !(t > 0.0f);
   Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
-  const Span sp = span_of(sh.nv, rank, cs);
-  sh.buf = row_smem;
-  sh.v0 = sp.v0;
-  sh.n = sp.v1 - sp.v0;
-  const FineScale f = greedy ? FineScale{0.0f, 0.0f} : fine_scale_of(t);
-  LaneStat st{-CUDART_INF_F, 0.0, INT32_MAX};
-  for (int i0 = 0; i0 < sh.n; i0 += U * kFThreads) {
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      raw[u] = load_vec(sh, sp.v0 + i0 + u * kFThreads + tid, sp.v1);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u * kFThreads + tid < sh.n)
-        row_smem[i0 + u * kFThreads + tid] = raw[u];
-    auto index = [&](int u) {
-      return sh.first(sp.v0 + i0 + u * kFThreads + tid);
-    };
-    if (greedy)
-      take_vecs<T, true, kNoSum>(raw, index, f, &ss.top, st);
-    else
-      take_vecs<T, false, kFineSum>(raw, index, f, &ss.top, st);
-  }
-  st.s = warp_sum64(st.s);
-  if (lane_id() == 0) ss.part[warp_id()] = SpanSum{st.s, st.m, st.arg};
-  __syncthreads();
-  if (warp_id() == 0) {
-    const SpanSum p = join_sums(ss.part, kFWarps, t);
-    if (lane_id() < cs) *cl.map_shared_rank(&ss.slot[rank], lane_id()) = p;
-  }
-  cl.sync();
-  const SpanSum row = join_sums(ss.slot, cs, t);
+  const SpanSum row = load_row(cl, sh, row_smem, t, rs);
   float* orow = a.out + r * a.rows.vocab;
-  if (greedy || !(row.m > -CUDART_INF_F))
-    write_one_hot(sh, orow, row.m > -CUDART_INF_F ? row.arg : -1);
+  if (!(row.m > -CUDART_INF_F))
+    write_one_hot(sh, orow, -1);
+  else if (!(t > 0.0f))
+    write_one_hot(sh, orow, row.arg);
   else
     write_kept<T, true>(sh, orow, row.m, -CUDART_INF_F, row.s, t);
 }
@@ -802,7 +881,7 @@ __global__ void __launch_bounds__(kFThreads, kKeptBlocks) stat_rows_kernel(RowAr
   FilterShared* fs = reinterpret_cast<FilterShared*>(row_smem);
   uint4* buf = row_smem + (sizeof(FilterShared) + 15) / 16;
   fill_exp_table(rs.tab);
-  __syncthreads();
+  if (threadIdx.x == 0) rs.top = 0;
   const int cs = static_cast<int>(cl.num_blocks());
   const bool leader = cl.block_rank() == 0;
   const int k = a.rows.positions - 1;
@@ -822,7 +901,7 @@ __global__ void __launch_bounds__(kFThreads, kKeptBlocks) stat_rows_kernel(RowAr
     const Setting set = setting_of(a.set, b);
     const T* row = row_ptr<T>(a.rows, b, j);
     Share<T> sh(row, a.rows.vocab);
-    const Kept kept = keep_row(cl, sh, buf, set, rs, *fs);
+    const Kept kept = keep_row(cl, sh, buf, set, a.guard, rs, *fs);
     if (leader && threadIdx.x == 0) {
       RowStat st;
       st.z = kept.z;
@@ -868,10 +947,11 @@ static int row_cluster(const sg_rows& r) {
 }
 
 template <class Kernel>
-static int launch_rows(Kernel* kernel, const RowArgs& a, bool filter,
-                       int64_t most, int* cache, cudaStream_t st) {
+static int launch_rows(Kernel* kernel, RowArgs& a, bool filter, int64_t most,
+                       int* cache, cudaStream_t st) {
   const int cs = row_cluster(a.rows);
   const int elems = a.rows.dtype == SG_F32 ? 4 : 8;
+  a.guard = guard_of(a.rows.vocab, 4 * kFThreads * cs * elems);
   const int64_t vecs = ceil_div(ceil_div(a.rows.vocab + elems - 1, elems), cs);
   const int64_t bytes =
       16 * vecs + (filter ? (sizeof(FilterShared) + 15) / 16 * 16 : 0);
@@ -888,7 +968,7 @@ static int launch_rows(Kernel* kernel, const RowArgs& a, bool filter,
 }
 
 template <class T>
-static int write_rows(const RowArgs& a, bool filter, cudaStream_t st) {
+static int write_rows(RowArgs& a, bool filter, cudaStream_t st) {
   static int cache[2][64];
   return filter ? launch_rows(kept_rows_kernel<T>, a, true, INT32_MAX,
                               cache[1], st)
@@ -897,7 +977,7 @@ static int write_rows(const RowArgs& a, bool filter, cudaStream_t st) {
 }
 
 template <class T>
-static int stat_rows(const RowArgs& a, cudaStream_t st) {
+static int stat_rows(RowArgs& a, cudaStream_t st) {
   static int cache[64];
   return launch_rows(stat_rows_kernel<T>, a, true, kKeptBlocks * 148, cache,
                      st);

@@ -3,7 +3,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "sg_sampling.cuh"
 
@@ -130,21 +129,6 @@ __device__ __forceinline__ RowSum join_parts(const Part* parts, int n,
   if (kSum) r.s = warp_sum64(r.s);
   if (kArg) r.arg = __reduce_min_sync(SG_FULL_MASK, arg);
   return r;
-}
-
-// A weight's relative error is 3 * 2^-24 * ln2 = 1.24e-7 times its depth z
-// (its exponent of 2) plus 2^-22: at most kDeepGuard for one weight, whose
-// depth ends at 126. In a row's sum it counts by weight, and the weights'
-// mean depth is at most log2(V): it is their entropy less log2 of their sum,
-// and the largest weight is 1. Further errors: 2^-22 for each time the
-// largest value grew (at most once a tile) or spans were joined (2), and
-// 2^-24 for each of the at most 20 fp32 operations on a weight's way.
-constexpr double kDeepGuard = 1.7e-5;
-static double guard_of(int64_t vocab, int elems, int spans) {
-  const int64_t tile = static_cast<int64_t>(kUnroll) * 32 * elems;
-  const int64_t tiles = ceil_div(vocab, spans * tile) + 1;
-  return 1.25e-7 * std::log2(static_cast<double>(vocab) + 1.0) +
-         2.4e-7 * static_cast<double>(2 + tiles) + 1.2e-6;
 }
 
 // Spans of a warp, so that a span is one or two tiles.
@@ -1021,7 +1005,7 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
     const int elems = logits->dtype == SG_F32 ? 4 : 8;
     va.warp_spans = warp_spans_of(logits->vocab, elems, va.split);
     const int spans = va.split * kSWarps * va.warp_spans;
-    va.guard = guard_of(logits->vocab, elems, spans);
+    va.guard = guard_of(logits->vocab, kUnroll * 32 * elems * spans);
     int32_t* ctl = reinterpret_cast<int32_t*>(va.parts + rows * spans);
     size_t zero = 0;
     if (sampling && logits->batch > kWholeBatch) {
