@@ -15,7 +15,8 @@ namespace sg {
 constexpr int kFThreads = 256;
 constexpr int kFWarps = kFThreads / 32;
 constexpr int kSoftBlocks = 5;  // blocks on an SM, plain softmax
-constexpr int kKeptBlocks = 3;  // and with filters
+constexpr int kKeptBlocks = 3;  // with filters
+constexpr int kStatBlocks = 4;  // with filters, nothing written
 constexpr int kBins = 1024;      // of a window; the last takes the rest
 constexpr float kPlaces = 64.0f;  // places told apart in a bin
 constexpr int kWindows = 4;      // looked at before bisect_row
@@ -61,13 +62,13 @@ struct FilterShared {
   int32_t n[kMaxCluster];
   uint32_t nall[kMaxCluster];
   double a[kMaxCluster];
-  uint64_t redl[kFWarps];
+  uint64_t redl[2][kFWarps];
   Plan plan;
   // first block, over the windows so far
   int32_t seen;          // values in earlier windows
   float mass;            // and their weights, about
-  int32_t k_found, pick;
-  float need;
+  int32_t k_found, pick, pick_most;
+  float need, need_most;  // top-p's share, with fewest and most values kept
   // the result; done 0: bisect_row, 2: sum the row exactly and come again
   double z;
   float low;
@@ -98,15 +99,33 @@ __device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* red) {
   v = lane_id() < kFWarps ? red[lane_id()] : 0u;
   return __reduce_max_sync(SG_FULL_MASK, v);
 }
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(SG_FULL_MASK, v, o);
+// The first block's sums over its candidates: one barrier each, `turn`
+// alternating between two sets of slots.
+__device__ __forceinline__ int32_t turn_sum_i32(int32_t v, int& turn,
+                                                uint64_t (*red)[kFWarps]) {
+  v = __reduce_add_sync(SG_FULL_MASK, v);
+  turn ^= 1;
+  if (lane_id() == 0) red[turn][warp_id()] = static_cast<uint32_t>(v);
   __syncthreads();
-  if (lane_id() == 0) red[warp_id()] = v;
+  uint32_t s = 0;
+#pragma unroll
+  for (int i = 0; i < kFWarps; ++i) s += static_cast<uint32_t>(red[turn][i]);
+  return static_cast<int32_t>(s);
+}
+// v < 2^49: two parts, whose warp sums fit 32 bits.
+__device__ __forceinline__ uint64_t turn_sum_u64(uint64_t v, int& turn,
+                                                 uint64_t (*red)[kFWarps]) {
+  const uint32_t lo = __reduce_add_sync(
+      SG_FULL_MASK, static_cast<uint32_t>(v) & 0xffffffu);
+  const uint32_t hi =
+      __reduce_add_sync(SG_FULL_MASK, static_cast<uint32_t>(v >> 24));
+  turn ^= 1;
+  if (lane_id() == 0)
+    red[turn][warp_id()] = (static_cast<uint64_t>(hi) << 24) + lo;
   __syncthreads();
   uint64_t s = 0;
 #pragma unroll
-  for (int i = 0; i < kFWarps; ++i) s += red[i];
+  for (int i = 0; i < kFWarps; ++i) s += red[turn][i];
   return s;
 }
 
@@ -263,7 +282,9 @@ __device__ __forceinline__ void plan_window(
   const int tid = static_cast<int>(threadIdx.x);
   int32_t c[kPer] = {0, 0, 0, 0};
   float o[kPer] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int r = 0; r < cs; ++r) {
+#pragma unroll 4
+  for (int r = 0; r < kMaxCluster; ++r) {
+    if (r >= cs) break;
     const FilterShared* from = cl.map_shared_rank(&fs, r);
     const uint4 h = reinterpret_cast<const uint4*>(from->hist)[tid];
     const uint4 f = reinterpret_cast<const uint4*>(from->offs)[tid];
@@ -299,7 +320,7 @@ __device__ __forceinline__ void plan_window(
     rs.redf[warp_id()] = mi;
   }
   if (tid == 0) {
-    fs.pick = INT32_MAX;
+    fs.pick = fs.pick_most = INT32_MAX;
     if (off == 0 && !fs.k_found) {
       fs.seen = 0;
       fs.mass = 0.0f;
@@ -330,13 +351,15 @@ __device__ __forceinline__ void plan_window(
         plan.bk = off + tid * kPer + i;
         plan.above = r;
         fs.pick = plan.bk;
+        // values equal to the k-th are kept too: up to the whole bin
         fs.need = p * (q + static_cast<float>(k - r) * w[i]);
+        fs.need_most = p * (q + static_cast<float>(c[i]) * w[i]);
       }
       r += c[i];
       q += static_cast<float>(c[i]) * w[i];
     }
   }
-  if (k <= 0 && tid == 0) fs.need = p * row_sum;
+  if (k <= 0 && tid == 0) fs.need = fs.need_most = p * row_sum;
   __syncthreads();
   bool k_now = false;
   if (k > 0 && !fs.k_found) {
@@ -355,23 +378,31 @@ __device__ __forceinline__ void plan_window(
       next = 0;  // it may lie in an earlier window
     } else {
       float q = mr;
-      int32_t at = INT32_MAX;
+      int32_t at = INT32_MAX, most = INT32_MAX;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         q += static_cast<float>(c[i]) * w[i];
-        if (q >= fs.need && tid * kPer + i < kBins - 1)
-          at = min(at, off + tid * kPer + i);
+        if (tid * kPer + i < kBins - 1) {
+          if (q >= fs.need) at = min(at, off + tid * kPer + i);
+          if (q >= fs.need_most) most = min(most, off + tid * kPer + i);
+        }
       }
       if (at != INT32_MAX) atomicMin(&fs.pick, at);
+      if (most != INT32_MAX) atomicMin(&fs.pick_most, most);
       __syncthreads();
       at = fs.pick;
+      most = fs.pick_most;
       // the border does not lie beyond the k-th value
-      if (k > 0 && plan.bk < off + kBins - 1) at = min(at, plan.bk);
-      if (at == INT32_MAX) {
+      if (k > 0 && plan.bk < off + kBins - 1) {
+        at = min(at, plan.bk);
+        most = min(most, plan.bk);
+      }
+      if (most == INT32_MAX) {
         next = off + kBins - 1;
+        if (at != INT32_MAX) next = kWindows * kBins;  // split: bisect_row
       } else if (tid == 0) {
         plan.p0 = max(at - 1, 0);
-        plan.p1 = k > 0 ? min(at + 1, plan.bk) : at + 1;
+        plan.p1 = k > 0 ? min(most + 1, plan.bk) : most + 1;
       }
     }
   } else if (k > 0 && !fs.k_found) {
@@ -486,6 +517,7 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
       }
       if (!exact) kept = row_sum;
       int done = fits && n <= kList;
+      int turn = 0;
       float low = -CUDART_INF_F;
       if (done) {
         // this thread's candidates: their keys, bins and fixed-point weights
@@ -539,7 +571,7 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
             int32_t c = 0;
 #pragma unroll
             for (int i = 0; i < kOwn; ++i) c += in_k[i] && key[i] >= from;
-            return block_sum_i32(c, rs.redi) >= want;
+            return turn_sum_i32(c, turn, fs.redl) >= want;
           });
           uint64_t f = 0;
 #pragma unroll
@@ -547,7 +579,7 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
             f += in_k[i] && key[i] >= tk ? w[i] : 0;
             in_p[i] = in_p[i] && key[i] >= tk;
           }
-          kept += static_cast<double>(block_sum_u64(f, fs.redl)) / kFix;
+          kept += static_cast<double>(turn_sum_u64(f, turn, fs.redl)) / kFix;
           low = key_value(tk);
         }
         if (with_p) {
@@ -558,7 +590,7 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
 #pragma unroll
             for (int i = 0; i < kOwn; ++i)
               f += in_p[i] && key[i] >= from ? w[i] : 0;
-            return a + static_cast<double>(block_sum_u64(f, fs.redl)) / kFix;
+            return a + static_cast<double>(turn_sum_u64(f, turn, fs.redl)) / kFix;
           };
           if (!(a < need - slack && mass(0) >= need + slack)) {
             done = exact ? 0 : 2;
@@ -873,7 +905,7 @@ __device__ __forceinline__ int64_t next_row(const RowArgs& a, RowQueue& q) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(kFThreads, kKeptBlocks) stat_rows_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kFThreads, kStatBlocks) stat_rows_kernel(RowArgs a) {
   const auto cl = cooperative_groups::this_cluster();
   __shared__ RowShared rs;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -979,7 +1011,7 @@ static int write_rows(RowArgs& a, bool filter, cudaStream_t st) {
 template <class T>
 static int stat_rows(RowArgs& a, cudaStream_t st) {
   static int cache[64];
-  return launch_rows(stat_rows_kernel<T>, a, true, kKeptBlocks * 148, cache,
+  return launch_rows(stat_rows_kernel<T>, a, true, kStatBlocks * 148, cache,
                      st);
 }
 
