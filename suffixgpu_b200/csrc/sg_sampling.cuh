@@ -14,14 +14,10 @@
 
 namespace sg {
 
-// One row's sampling statistics, written per (request, position) by the
-// statistics kernels and read by the kernels that pick or write.
+// What a verification with top-k or top-p knows of a row.
 struct RowStat {
-  double z;       // sum of the kept weights, relative to the largest value
-  float m;         // largest value of the row
-  int32_t arg;     // its lowest index (greedy rows), -1: no mass
-  float low;       // smallest kept value
-  int32_t accept;  // 1: this position's draft is accepted
+  int32_t token;   // what follows if the row's draft is not accepted, -1: none
+  int32_t accept;  // 1: it is
 };
 
 // Row `j` of request `b`, or null when the request has no such row.
@@ -631,8 +627,8 @@ __device__ __forceinline__ Pick pick_span(int spans, double u, SumOf sum_of) {
 // that owns the span with the target scans it. Called by every thread of
 // the cluster, same result in all.
 //   Src::E              weights of a vector
-//   src.nv              vectors
 //   src.first(v)        index of a vector's first weight
+//   src.span(w, n)      vectors of span w of n = 8 a block, in order
 //   src.sum(v, end, st) sum of the weights of vectors v, v + st, ... < end
 //   src.vec(v, end, w)  weights of vector v
 struct DrawShared {
@@ -648,7 +644,7 @@ __device__ int32_t cluster_draw(const cooperative_groups::cluster_group& cl,
   const int rank = static_cast<int>(cl.block_rank());
   const int spans = cs * kCWarps;
   const int mine = rank * kCWarps + warp_id();
-  const Span sp = span_of(src.nv, mine, spans);
+  const Span sp = src.span(mine, spans);
   const double s = warp_sum64(src.sum(sp.v0 + lane_id(), sp.v1, 32));
   cl.sync();  // sh is free
   if (lane_id() < cs) *cl.map_shared_rank(&sh.seg[mine], lane_id()) = s;
@@ -657,7 +653,7 @@ __device__ int32_t cluster_draw(const cooperative_groups::cluster_group& cl,
   if (pick.span < 0) return -1;
   if (pick.span / kCWarps == rank) {
     // a contiguous run of vectors a thread
-    const Span seg = span_of(src.nv, pick.span, spans);
+    const Span seg = src.span(pick.span, spans);
     const int per = (seg.v1 - seg.v0 + kCThreads - 1) / kCThreads;
     const int v0 = min(seg.v1, seg.v0 + static_cast<int>(threadIdx.x) * per);
     const int v1 = min(seg.v1, v0 + per);

@@ -16,7 +16,7 @@ constexpr int kFThreads = 256;
 constexpr int kFWarps = kFThreads / 32;
 constexpr int kSoftBlocks = 5;  // blocks on an SM, plain softmax
 constexpr int kKeptBlocks = 3;  // with filters
-constexpr int kStatBlocks = 4;  // with filters, nothing written
+constexpr int kStatBlocks = 2;  // with filters, nothing written
 constexpr int kBins = 1024;      // of a window; the last takes the rest
 constexpr float kPlaces = 64.0f;  // places told apart in a bin
 constexpr int kWindows = 4;      // looked at before bisect_row
@@ -440,8 +440,8 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
   const int rank = static_cast<int>(cl.block_rank());
   const int tid = static_cast<int>(threadIdx.x);
   const bool with_p = p < 1.0f;
-  // 64 bins an octave of weight, 96 a unit of logits at least
-  sh.bin_scale = fminf(fmaxf(64.0f * sh.scale, 96.0f), 1e30f);
+  // 16 bins an octave of weight, 96 a unit of logits at least
+  sh.bin_scale = fminf(fmaxf(16.0f * sh.scale, 96.0f), 1e30f);
   if (tid == 0) {
     fs.listed = 0;
     fs.k_found = 0;
@@ -624,12 +624,12 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
 }
 
 // Loads a row's shares into shared memory and gives its largest value, the
-// lowest index of that (t not > 0) or the fp32 sum of its weights (t > 0):
+// lowest index of that (t not > 0) or the fp32 sum of its weights (with_sum):
 // a running maximum a warp, one exchange over the cluster. rs.top is 0.
 template <class T>
 __device__ __forceinline__ SpanSum
 load_row(const cooperative_groups::cluster_group& cl, Share<T>& sh, uint4* buf,
-         float t, RowShared& rs) {
+         float t, bool with_sum, RowShared& rs) {
   constexpr int U = 4;
   const int cs = static_cast<int>(cl.num_blocks());
   const int rank = static_cast<int>(cl.block_rank());
@@ -655,10 +655,12 @@ load_row(const cooperative_groups::cluster_group& cl, Share<T>& sh, uint4* buf,
     };
     if (greedy)
       take_vecs<T, true, kNoSum>(raw, index, f, &rs.top, st);
-    else
+    else if (with_sum)
       take_vecs<T, false, kFineSum>(raw, index, f, &rs.top, st);
+    else
+      take_vecs<T, false, kNoSum>(raw, index, f, &rs.top, st);
   }
-  st.s = warp_sum64(st.s);
+  if (with_sum) st.s = warp_sum64(st.s);
   if (lane_id() == 0) rs.part[warp_id()] = SpanSum{st.s, st.m, st.arg};
   __syncthreads();
   if (warp_id() == 0) {
@@ -681,7 +683,11 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
   const int rank = static_cast<int>(cl.block_rank());
   const int tid = static_cast<int>(threadIdx.x);
   for (int i = tid; i < kBins; i += kFThreads) fs.hist[i] = fs.offs[i] = 0;
-  const SpanSum row = load_row(cl, sh, buf, set.t, rs);
+  const int32_t k = set.k > 0 && set.k < sh.v ? set.k : 0;
+  const float p = set.p < 1.0f ? set.p : 1.0f;
+  // the row's sum is what top-p without top-k takes its share of
+  const SpanSum row =
+      load_row(cl, sh, buf, set.t, set.t > 0.0f && k == 0 && p < 1.0f, rs);
   Kept kept{0.0, row.m, -CUDART_INF_F, -1};
   if (!(row.m > -CUDART_INF_F)) return kept;  // no mass
   kept.arg = 0;
@@ -695,8 +701,6 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
   sh.scale = scale_of(set.t);
   sh.scale64 = scale64_of(set.t);
   sh.tab = rs.tab;
-  const int32_t k = set.k > 0 && set.k < sh.v ? set.k : 0;
-  const float p = set.p < 1.0f ? set.p : 1.0f;
   double s = 0.0;
   if (row.m == CUDART_INF_F || !(p > 0.0f)) {
     // only the largest value has mass, or is kept
@@ -854,7 +858,7 @@ __global__ void __launch_bounds__(kFThreads, kSoftBlocks)
   const int j = static_cast<int>(r % a.rows.positions);
   const float t = setting_of(a.set, b).t;
   Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
-  const SpanSum row = load_row(cl, sh, row_smem, t, rs);
+  const SpanSum row = load_row(cl, sh, row_smem, t, t > 0.0f, rs);
   float* orow = a.out + r * a.rows.vocab;
   if (!(row.m > -CUDART_INF_F))
     write_one_hot(sh, orow, -1);
@@ -904,10 +908,61 @@ __device__ __forceinline__ int64_t next_row(const RowArgs& a, RowQueue& q) {
   }
 }
 
+// Exact weights of a row's kept values, without token `skip`, from the blocks'
+// shares: cluster_draw's source. Weights are formed only where a vector holds
+// such a value.
 template <class T>
-__global__ void __launch_bounds__(kFThreads, kStatBlocks) stat_rows_kernel(RowArgs a) {
+struct KeptShare {
+  static constexpr int E = Share<T>::E;
+  const Share<T>& sh;
+  float low;
+  int64_t skip;
+
+  __device__ __forceinline__ int64_t first(int v) const { return sh.first(v); }
+  __device__ __forceinline__ Span span(int w, int n) const {
+    const Span block = span_of(sh.nv, w / kCWarps, n / kCWarps);
+    Span s = span_of(block.v1 - block.v0, w % kCWarps, kCWarps);
+    s.v0 += block.v0;
+    s.v1 += block.v0;
+    return s;
+  }
+  __device__ __forceinline__ double value_weight(float x) const {
+    if (!(x >= low)) return 0.0;
+    return x == sh.m ? 1.0 : sh.weight(x);
+  }
+  __device__ __forceinline__ void vec(int v, int, double* w) const {
+    const uint4 raw[1] = {sh.buf[v - sh.v0]};
+    float x[E];
+    Raw<T>::unpack(raw[0], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = 0.0;
+    if (!(Raw<T>::vec_max(raw) >= low)) return;
+    const int64_t at = first(v);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (at + e != skip) w[e] = value_weight(x[e]);
+  }
+  __device__ __forceinline__ double sum(int v, int end, int step) const {
+    double s = 0.0;
+    for (; v < end; v += step) {
+      const uint4 raw[1] = {sh.buf[v - sh.v0]};
+      if (!(Raw<T>::vec_max(raw) >= low)) continue;
+      double w[E];
+      vec(v, end, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += w[e];
+    }
+    return s;
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kFThreads, kStatBlocks)
+    stat_rows_kernel(RowArgs a) {
+  static_assert(kFThreads == kCThreads, "cluster_draw's blocks");
   const auto cl = cooperative_groups::this_cluster();
   __shared__ RowShared rs;
+  __shared__ DrawShared ds;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   FilterShared* fs = reinterpret_cast<FilterShared*>(row_smem);
@@ -934,29 +989,33 @@ __global__ void __launch_bounds__(kFThreads, kStatBlocks) stat_rows_kernel(RowAr
     const T* row = row_ptr<T>(a.rows, b, j);
     Share<T> sh(row, a.rows.vocab);
     const Kept kept = keep_row(cl, sh, buf, set, a.guard, rs, *fs);
-    if (leader && threadIdx.x == 0) {
-      RowStat st;
-      st.z = kept.z;
-      st.m = kept.m;
-      st.arg = kept.arg;
-      st.low = kept.low;
-      st.accept = 0;
-      const int32_t x =
-          j < k ? a.draft[static_cast<int64_t>(b) * k + j] : -1;
-      if (x >= 0 && x < a.rows.vocab && kept.arg >= 0) {
-        const double u = a.uniforms[static_cast<int64_t>(b) * (k + 1) + j];
-        if (!(set.t > 0.0f)) {
-          st.accept = x == kept.arg && u < 1.0;
-        } else {
-          const float l = canon(to_f32(row[x]));
-          double w = 0.0;
-          if (l >= kept.low)
-            w = l == kept.m ? 1.0
-                            : weight64(l, static_cast<double>(kept.m),
-                                       scale64_of(set.t), rs.tab);
-          st.accept = u < w / kept.z;
+    // Every block comes to the same verdict. The token that follows if the
+    // draft is not accepted is drawn while the row is at hand.
+    const int n = valid_drafts(a.num_valid, b, k);
+    const float* urow = a.uniforms + static_cast<int64_t>(b) * (k + 1);
+    const int32_t x = j < n ? a.draft[static_cast<int64_t>(b) * k + j] : -1;
+    RowStat st{kept.arg, 0};
+    if (kept.arg >= 0) {
+      const bool greedy = !(set.t > 0.0f);
+      const bool inside = x >= 0 && x < a.rows.vocab;
+      const double u = inside ? urow[j] : 0.0f;
+      if (greedy) {
+        st.accept = inside && x == kept.arg && u < 1.0;
+      } else {
+        KeptShare<T> src{sh, kept.low, x};
+        if (inside)
+          st.accept =
+              u < src.value_weight(canon(to_f32(row[x]))) / kept.z;
+        if (!st.accept) {
+          st.token = cluster_draw(cl, src, urow[k], ds);
+          if (st.token < 0) {  // nothing but the rejected token
+            src.skip = -1;
+            st.token = cluster_draw(cl, src, urow[k], ds);
+          }
         }
       }
+    }
+    if (leader && threadIdx.x == 0) {
       a.stats[static_cast<int64_t>(b) * (k + 1) + j] = st;
       if (!st.accept && j < k) atomicMax(a.rejected + b, k + 1 - j);
     }
@@ -966,31 +1025,35 @@ __global__ void __launch_bounds__(kFThreads, kStatBlocks) stat_rows_kernel(RowAr
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Blocks a row is split over: shares of at most 32 KiB (more blocks on an
-// SM), but enough blocks to fill the machine where rows are few.
-static int row_cluster(const sg_rows& r) {
+// Blocks a row is split over: shares of at most `share` bytes, but enough
+// blocks to fill the machine where rows are few. 32 KiB where rows are
+// written; 64 KiB for the statistics, whose passes cost every block much the
+// same whatever its share (128 x 33 rows of 128256 bf16, top-k and top-p:
+// 371 us against 504, and 566 with 128 KiB).
+static int row_cluster(const sg_rows& r, int64_t share) {
   const int64_t rows = static_cast<int64_t>(r.batch) * r.positions;
   const int64_t bytes = r.vocab * (r.dtype == SG_F32 ? 4 : 2);
   int cs = 1;
   while (cs < kMaxCluster &&
-         (bytes > cs * 32768 || (rows * cs < 148 && bytes > cs * 4096)))
+         (bytes > cs * share || (rows * cs < 148 && bytes > cs * 4096)))
     cs *= 2;
   return cs;
 }
 
 template <class Kernel>
-static int launch_rows(Kernel* kernel, RowArgs& a, bool filter, int64_t most,
-                       int* cache, cudaStream_t st) {
-  const int cs = row_cluster(a.rows);
+static int launch_rows(Kernel* kernel, RowArgs& a, bool filter, int64_t share,
+                       int64_t most, int* cache, cudaStream_t st) {
+  const int cs = row_cluster(a.rows, share);
   const int elems = a.rows.dtype == SG_F32 ? 4 : 8;
   a.guard = guard_of(a.rows.vocab, 4 * kFThreads * cs * elems);
   const int64_t vecs = ceil_div(ceil_div(a.rows.vocab + elems - 1, elems), cs);
   const int64_t bytes =
       16 * vecs + (filter ? (sizeof(FilterShared) + 15) / 16 * 16 : 0);
   if (bytes > 200 * 1024) return SG_ERR_UNSUPPORTED;
-  // 1 KiB more: the static shared memory counts towards the same limit
+  // 2 KiB more: the static shared memory counts towards the same limit
+  static_assert(sizeof(RowShared) + sizeof(DrawShared) <= 2048, "");
   const int rc =
-      ensure_dyn_smem(kernel, static_cast<size_t>(bytes) + 1024, cache);
+      ensure_dyn_smem(kernel, static_cast<size_t>(bytes) + 2048, cache);
   if (rc != SG_OK) return rc;
   const int64_t rows = static_cast<int64_t>(a.rows.batch) * a.rows.positions;
   if (rows > INT32_MAX / kMaxCluster) return SG_ERR_UNSUPPORTED;
@@ -1002,17 +1065,17 @@ static int launch_rows(Kernel* kernel, RowArgs& a, bool filter, int64_t most,
 template <class T>
 static int write_rows(RowArgs& a, bool filter, cudaStream_t st) {
   static int cache[2][64];
-  return filter ? launch_rows(kept_rows_kernel<T>, a, true, INT32_MAX,
-                              cache[1], st)
-                : launch_rows(soft_rows_kernel<T>, a, false, INT32_MAX,
-                              cache[0], st);
+  return filter ? launch_rows(kept_rows_kernel<T>, a, true, 32768,
+                              INT32_MAX, cache[1], st)
+                : launch_rows(soft_rows_kernel<T>, a, false, 32768,
+                              INT32_MAX, cache[0], st);
 }
 
 template <class T>
 static int stat_rows(RowArgs& a, cudaStream_t st) {
   static int cache[64];
-  return launch_rows(stat_rows_kernel<T>, a, true, kStatBlocks * 148, cache,
-                     st);
+  return launch_rows(stat_rows_kernel<T>, a, true, 65536,
+                     kStatBlocks * 148, cache, st);
 }
 
 int launch_row_stats(const sg_rows& rows, const sg_sampling& set,

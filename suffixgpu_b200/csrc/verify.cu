@@ -288,6 +288,9 @@ struct RowWeights : RowVecs<T> {
     }
   }
   // Exact weights (cluster_draw's source).
+  __device__ __forceinline__ Span span(int w, int n) const {
+    return span_of(this->nv, w, n);
+  }
   __device__ __forceinline__ void vec(int v, int end, double* w) const {
     exact(load_vec(*this, v, end), v, w);
   }
@@ -601,96 +604,29 @@ static int split_of(int64_t rows) {
 // ---------------------------------------------------------------------------
 // verification from logits with top-k or top-p
 // ---------------------------------------------------------------------------
-// The rows' statistics hold the smallest kept value, the kept mass and the
-// verdict on each draft (target_probs.cu); one cluster a request draws.
-struct PickArgs {
-  sg_rows rows;
-  sg_sampling set;
+// The rows' kernel (target_probs.cu) has left the verdict on each draft and
+// the token that follows a rejection; a warp a request puts them together.
+struct GatherArgs {
   const RowStat* stats;
   const int32_t* draft;
   const int32_t* num_valid;
-  const float* uniforms;
   int32_t* sampled;
   int32_t* count;
+  int32_t batch;
+  int32_t k;
 };
 
-// Exact weights of the values >= low, without token `skip`; weights are
-// formed only where a vector holds such a value.
-template <class T>
-struct KeptWeights : RowVecs<T> {
-  using RowVecs<T>::E;
-  float m, low;
-  double scale64;
-  int64_t skip;
-  const double* tab;
-
-  __device__ __forceinline__ KeptWeights(const T* row, int64_t vocab)
-      : RowVecs<T>(row, vocab) {}
-  __device__ __forceinline__ bool exact(const uint4& raw, int v,
-                                        double* w) const {
-    float x[E];
-    Raw<T>::unpack(raw, x);
-    bool any = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) any = any || x[e] >= low;
-#pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = 0.0;
-    if (!any) return false;
-    const int64_t i0 = this->first(v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (x[e] >= low && i0 + e != skip)
-        w[e] = x[e] == m ? 1.0
-                         : weight64(x[e], static_cast<double>(m), scale64,
-                                    tab);
-    }
-    return true;
-  }
-  __device__ __forceinline__ void vec(int v, int end, double* w) const {
-    exact(load_vec(*this, v, end), v, w);
-  }
-  __device__ __forceinline__ double sum(int v, int end, int step) const {
-    constexpr int U = 4;  // loads in flight
-    double s = 0.0;
-    for (; v < end; v += U * step) {
-      uint4 raw[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = load_vec(*this, v + u * step, end);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        double w[E];
-        if (exact(raw[u], v + u * step, w)) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) s += w[e];
-        }
-      }
-    }
-    return s;
-  }
-};
-
-template <class T>
-__global__ void __launch_bounds__(kCThreads) pick_kernel(PickArgs a) {
-  const auto cl = cooperative_groups::this_cluster();
-  __shared__ DrawShared sh;
-  __shared__ double s_tab[kExpTable];
+__global__ void __launch_bounds__(kCThreads) gather_kernel(GatherArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  fill_exp_table(s_tab);
-  __syncthreads();
-  const int b = static_cast<int>(blockIdx.x / cl.num_blocks());
-  const bool leader = cl.block_rank() == 0;
-  const int k = a.rows.positions - 1;
-  const int n = valid_drafts(a.num_valid, b, k);
-  const int32_t* drow = a.draft + static_cast<int64_t>(b) * k;
-  int32_t* out = a.sampled + static_cast<int64_t>(b) * (k + 1);
-  if (n < 0) {  // the whole cluster leaves: no barrier is waited for
-    if (leader) emit(drow, 0, -1, k, out, a.count + b);
-    return;
-  }
-  const RowStat* stats = a.stats + static_cast<int64_t>(b) * (k + 1);
-  int s = 0;
-  for (int j0 = 0;; j0 += 32) {
+  const int b = static_cast<int>(blockIdx.x) * kCWarps + warp_id();
+  if (b >= a.batch) return;
+  const int n = valid_drafts(a.num_valid, b, a.k);
+  const RowStat* stats = a.stats + static_cast<int64_t>(b) * (a.k + 1);
+  const int32_t* drow = a.draft + static_cast<int64_t>(b) * a.k;
+  int32_t* out = a.sampled + static_cast<int64_t>(b) * (a.k + 1);
+  int s = n;  // -1: inactive
+  for (int j0 = 0; j0 < n; j0 += 32) {
     const int j = j0 + lane_id();
     const unsigned no =
         __ballot_sync(SG_FULL_MASK, j >= n || !stats[j].accept);
@@ -699,31 +635,10 @@ __global__ void __launch_bounds__(kCThreads) pick_kernel(PickArgs a) {
       break;
     }
   }
-  const RowStat st = stats[s];
-  int32_t tok = st.arg;
-  const Setting set = setting_of(a.set, b);
-  if (st.arg >= 0 && set.t > 0.0f) {
-    const double u = a.uniforms[static_cast<int64_t>(b) * (k + 1) + k];
-    KeptWeights<T> weights(row_ptr<T>(a.rows, b, s), a.rows.vocab);
-    weights.m = st.m;
-    weights.low = st.low;
-    weights.scale64 = scale64_of(set.t);
-    weights.skip = s < n ? drow[s] : -1;
-    weights.tab = s_tab;
-    tok = cluster_draw(cl, weights, u, sh);
-    if (tok < 0) {  // nothing but the rejected token
-      weights.skip = -1;
-      tok = cluster_draw(cl, weights, u, sh);
-    }
-  }
-  if (leader) emit(drow, s, tok, k, out, a.count + b);
-}
-
-template <class T>
-static int launch_pick(const PickArgs& a, cudaStream_t st) {
-  return launch_after(pick_kernel<T>,
-                      static_cast<unsigned>(a.rows.batch) * kMaxCluster,
-                      kCThreads, kMaxCluster, a, st);
+  const int32_t tok = s >= 0 ? stats[s].token : -1;
+  for (int j = lane_id(); j <= a.k; j += 32)
+    out[j] = j < s ? drow[j] : (j == s ? tok : -1);
+  if (lane_id() == 0) a.count[b] = max(s, 0) + (tok >= 0 ? 1 : 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -789,6 +704,9 @@ struct ProbWeights : RowVecs<float> {
       for (int e = 0; e < E; ++e)
         if (e == at) w[e] = 0.0;
     }
+  }
+  __device__ __forceinline__ Span span(int w, int n) const {
+    return span_of(nv, w, n);
   }
   __device__ __forceinline__ void vec(int at, int end, double* w) const {
     uint4 a, b;
@@ -1042,13 +960,12 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
   rc = launch_row_stats(*logits, *sampling, draft, num_valid, uniforms, stats,
                         rejected, rejected + logits->batch, st);
   if (rc != SG_OK) return rc;
-  const PickArgs pa{*logits,   *sampling, stats,   draft,
-                    num_valid, uniforms,  sampled, count};
-  switch (logits->dtype) {
-    case SG_F32: return launch_pick<float>(pa, st);
-    case SG_BF16: return launch_pick<__nv_bfloat16>(pa, st);
-    default: return launch_pick<__half>(pa, st);
-  }
+  const GatherArgs ga{stats, draft,         num_valid,
+                      sampled, count, logits->batch, logits->positions - 1};
+  return launch_after(
+      gather_kernel,
+      static_cast<unsigned>(ceil_div(logits->batch, kCWarps)), kCThreads, 1,
+      ga, st);
 }
 
 }  // namespace sg
