@@ -18,6 +18,7 @@
 // target_probs wrap the draft-verification entry points; their argument
 // checks run before any CUDA call (and raise ValueError).
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -28,6 +29,7 @@
 #include <cstring>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../include/suffixgpu.h"
@@ -444,11 +446,17 @@ sg_sampling sampling_of(const c10::optional<at::Tensor>& temperature,
   return s;
 }
 
+// An uninitialised tensor on the device of `like`, past the dispatcher.
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes,
+                    at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
+
 // What the three verify operators share: the checked index tensors, the
 // output buffer and the launch stream.
 struct VerifyCall {
   int64_t b = 0, k = 0;
-  at::Tensor draft, num_valid, row_start, uniforms, buf;
+  at::Tensor draft, num_valid, row_start, uniforms, ids, counts;
   const int32_t* draft_ptr = nullptr;
   const int32_t* nv_ptr = nullptr;
   int32_t* sampled = nullptr;
@@ -488,16 +496,16 @@ struct VerifyCall {
                       "suffixgpu_b200 ops need CUDA tensors");
     r->data = rows.data_ptr();
     if (row_start.defined()) r->row_start = row_start.data_ptr<int32_t>();
-    buf = at::empty({b * (k + 2)}, draft.options());
-    sampled = buf.data_ptr<int32_t>();
-    count = sampled + b * (k + 1);
+    ids = empty_on(rows, {b, k + 1}, at::kInt);
+    counts = empty_on(rows, {b}, at::kInt);
+    sampled = ids.data_ptr<int32_t>();
+    count = counts.data_ptr<int32_t>();
     draft_ptr = draft.data_ptr<int32_t>();
     if (num_valid.defined()) nv_ptr = num_valid.data_ptr<int32_t>();
   }
 
-  std::tuple<at::Tensor, at::Tensor> result() const {
-    return {buf.narrow(0, 0, b * (k + 1)).view({b, k + 1}),
-            buf.narrow(0, b * (k + 1), b)};
+  std::tuple<at::Tensor, at::Tensor> result() {
+    return {std::move(ids), std::move(counts)};
   }
 };
 
@@ -509,9 +517,10 @@ sg_stream_t stream_for(const at::Tensor& t) {
 // A workspace of the call's own: calls on other streams and other captured
 // graphs never share one.
 at::Tensor verify_workspace(const sg_rows& r, const at::Tensor& like) {
-  return at::empty({static_cast<int64_t>(
-                       sg_verify_workspace_size(r.batch, r.positions)) + 16},
-                   like.options().dtype(at::kByte));
+  return empty_on(like,
+                  {static_cast<int64_t>(
+                      sg_verify_workspace_size(r.batch, r.positions)) + 16},
+                  at::kByte);
 }
 
 std::tuple<at::Tensor, at::Tensor> verify_greedy(
@@ -609,7 +618,7 @@ at::Tensor target_probs(const at::Tensor& logits,
   TORCH_CHECK_VALUE(rows.is_cuda(), "suffixgpu_b200 ops need CUDA tensors");
   const c10::cuda::CUDAGuard guard(rows.device());
   r.data = rows.data_ptr();
-  at::Tensor out = at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
+  at::Tensor out = empty_on(logits, logits.sizes(), at::kFloat);
   check_status("sg_target_probs",
                sg_target_probs(&r, &s, out.data_ptr<float>(),
                                stream_for(rows)));

@@ -251,6 +251,18 @@ def longest_suffix_match(sa, corpus, query, query_len, max_len: int):
 # draft verification (no reference counterpart: the reference ends at the
 # drafts and takes the sampled ids back)
 # ---------------------------------------------------------------------------
+_verify_ops: dict = {}
+
+
+def _verify_op(name: str):
+    """The operator's overload itself: the call skips the look-up by name
+    and the choice of an overload (a microsecond or so)."""
+    op = _verify_ops.get(name)
+    if op is None:
+        op = _verify_ops[name] = getattr(torch_ops(), name).default
+    return op
+
+
 def _setting(value, off):
     """(tensor, number) of a per-request setting: one of the two is used."""
     if value is None:
@@ -278,7 +290,7 @@ def verify_greedy(logits: torch.Tensor, draft: torch.Tensor,
     Returns (sampled [B, K + 1] int32, -1 past the count; count [B] int32),
     what propose_with_update takes as its sampled ids and their count. A
     row with nothing but -inf ends its request without a token."""
-    return torch_ops().verify_greedy(logits, draft, num_valid, row_start)
+    return _verify_op("verify_greedy")(logits, draft, num_valid, row_start)
 
 
 def verify_sampled(logits: torch.Tensor, draft: torch.Tensor,
@@ -307,8 +319,8 @@ def verify_sampled(logits: torch.Tensor, draft: torch.Tensor,
     t, t_all = _setting(temperature, 1.0)
     k, k_all = _setting(top_k, 0)
     p, p_all = _setting(top_p, 1.0)
-    return torch_ops().verify_sampled(logits, draft, uniforms, num_valid, t,
-                                      k, p, t_all, k_all, p_all, row_start)
+    return _verify_op("verify_sampled")(logits, draft, uniforms, num_valid, t,
+                                        k, p, t_all, k_all, p_all, row_start)
 
 
 def verify_probs(probs: torch.Tensor, draft: torch.Tensor,
@@ -323,8 +335,8 @@ def verify_probs(probs: torch.Tensor, draft: torch.Tensor,
     uniforms[b, j] * q_j(x) < p_j(x), and the token after a rejection is
     drawn from max(p - q, 0). Values that are negative or not finite count
     as 0; a row without mass ends its request without a token."""
-    return torch_ops().verify_probs(probs, draft, uniforms, num_valid,
-                                    draft_probs, row_start)
+    return _verify_op("verify_probs")(probs, draft, uniforms, num_valid,
+                                      draft_probs, row_start)
 
 
 def target_probs(logits: torch.Tensor,
@@ -338,4 +350,4 @@ def target_probs(logits: torch.Tensor,
     t, t_all = _setting(temperature, 1.0)
     k, k_all = _setting(top_k, 0)
     p, p_all = _setting(top_p, 1.0)
-    return torch_ops().target_probs(logits, t, k, p, t_all, k_all, p_all)
+    return _verify_op("target_probs")(logits, t, k, p, t_all, k_all, p_all)

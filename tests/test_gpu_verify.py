@@ -415,6 +415,58 @@ def test_streams_graphs_and_repeats():
             assert torch.equal(out[2], wantp[(i + a) % 3])
 
 
+def test_vocabularies_beyond_shared_memory():
+    """Rows that do not fit a cluster's shared memory: refused where the row
+    has to be held, verified where it is only read through."""
+    v = 600_001
+    logits, draft, nv, u = _case(2, 2, 1, v, torch.float32)
+    _sampled(logits, draft, u, nv, 0.8)
+    d, n = _np(draft, nv)
+    _check(ops.verify_greedy(logits, draft, nv),
+           vo.verify_greedy(_f64(logits), d, n))
+    with pytest.raises(RuntimeError, match="beyond supported limits"):
+        ops.target_probs(logits)
+    with pytest.raises(RuntimeError, match="beyond supported limits"):
+        ops.verify_sampled(logits, draft, u, nv, 0.8, top_p=0.9)
+    half = logits.to(torch.bfloat16)
+    _sampled(half, draft, u, nv, 0.8, p=0.9)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("fill", ["equal", "two", "near", "ramp", "flat"])
+def test_filters_on_crowded_rows(fill, dtype):
+    """Many values at or next to the borders: all equal, two values, values
+    one step apart, a ramp far beyond the first bins, a wide flat row."""
+    v = 20_011
+    i = torch.arange(v, dtype=torch.float32)
+    g = torch.Generator().manual_seed(5)
+    row = {"equal": torch.full((v,), 2.5), "two": (i % 2) * 0.25,
+           "near": 8.0 + (i % 701) * 2.0 ** -20,
+           "ramp": -(i % 4999) * 0.03,
+           "flat": torch.randn(v, generator=g) * 0.5}[fill]
+    logits = row[torch.randperm(v, generator=g)].to(dtype)
+    logits = logits.expand(6, 2, v).contiguous().to(DEV)
+    t = torch.tensor([1.0, 0.3, 4.0, 60.0, 1.0, 0.05])
+    k = torch.tensor([0, 7, 3000, 0, 19_000, 500], dtype=torch.int32)
+    p = torch.tensor([0.9, 0.5, 0.97, 0.3, 1.0, 0.999])
+    args = (t.to(DEV), k.to(DEV), p.to(DEV))
+    # equal weights in the thousands: the fp32 sum's own rounding, 2^-24 for
+    # each of at most 20 additions, comes on top of _probs_close's 8
+    got = ops.target_probs(logits, *args)
+    x = _f64(logits)
+    for b in range(6):
+        want = vo.row_probs(x[b, 0], float(t[b]), int(k[b]), float(p[b]))
+        gb = got[b, 0].double().cpu().numpy()
+        # weights below 2^-126 may be flushed; dropped tokens are 0
+        assert (gb[want > 2.0 ** -125] > 0).all() and (gb[want == 0] == 0).all()
+        depth = np.abs(x[b, 0] - x[b, 0].max()) / float(t[b])
+        tol = 2.0 ** -24 * (3 * depth + 28) * want + 2.0 ** -126
+        assert (np.abs(gb - want) <= tol).all()
+    draft = torch.full((6, 1), 11, dtype=torch.int32, device=DEV)
+    u = torch.rand(6, 2, generator=g).to(DEV)
+    _sampled(logits, draft, u, None, *args)
+
+
 def test_refusals_on_the_gpu():
     logits, draft, nv, u = _case(1, 2, 2, 64, torch.float32)
     with pytest.raises(ValueError, match="another device"):
