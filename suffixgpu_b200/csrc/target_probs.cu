@@ -626,11 +626,10 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
 // Loads a row's shares into shared memory and gives its largest value, the
 // lowest index of that (t not > 0) or the fp32 sum of its weights (with_sum):
 // a running maximum a warp, one exchange over the cluster. rs.top is 0.
-template <class T>
+template <int U, class T>
 __device__ __forceinline__ SpanSum
 load_row(const cooperative_groups::cluster_group& cl, Share<T>& sh, uint4* buf,
          float t, bool with_sum, RowShared& rs) {
-  constexpr int U = 4;
   const int cs = static_cast<int>(cl.num_blocks());
   const int rank = static_cast<int>(cl.block_rank());
   const int tid = static_cast<int>(threadIdx.x);
@@ -687,7 +686,7 @@ __device__ Kept keep_row(const cooperative_groups::cluster_group& cl,
   const float p = set.p < 1.0f ? set.p : 1.0f;
   // the row's sum is what top-p without top-k takes its share of
   const SpanSum row =
-      load_row(cl, sh, buf, set.t, set.t > 0.0f && k == 0 && p < 1.0f, rs);
+      load_row<8>(cl, sh, buf, set.t, set.t > 0.0f && k == 0 && p < 1.0f, rs);
   Kept kept{0.0, row.m, -CUDART_INF_F, -1};
   if (!(row.m > -CUDART_INF_F)) return kept;  // no mass
   kept.arg = 0;
@@ -858,7 +857,7 @@ __global__ void __launch_bounds__(kFThreads, kSoftBlocks)
   const int j = static_cast<int>(r % a.rows.positions);
   const float t = setting_of(a.set, b).t;
   Share<T> sh(row_ptr<T>(a.rows, b, j), a.rows.vocab);
-  const SpanSum row = load_row(cl, sh, row_smem, t, t > 0.0f, rs);
+  const SpanSum row = load_row<4>(cl, sh, row_smem, t, t > 0.0f, rs);
   float* orow = a.out + r * a.rows.vocab;
   if (!(row.m > -CUDART_INF_F))
     write_one_hot(sh, orow, -1);
