@@ -100,6 +100,11 @@ __device__ __forceinline__ Part warp_stats(const RowVecs<T>& rv, Span sp,
   return Part{s, st.m, st.arg};
 }
 
+// Past the L1 cache: other blocks of the same launch may have written it.
+__device__ __forceinline__ Part load_part(const Part* p) {
+  return Part{__ldcg(&p->s), __ldcg(&p->m), __ldcg(&p->arg)};
+}
+
 // A row from the Parts of its `n` spans, in every lane of the warp.
 struct RowSum {
   double s;
@@ -115,7 +120,7 @@ __device__ __forceinline__ RowSum join_parts(const Part* parts, int n,
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     p[i] = Part{0.0f, -CUDART_INF_F, INT32_MAX};
-    if (i * 32 + lane_id() < n) p[i] = parts[i * 32 + lane_id()];
+    if (i * 32 + lane_id() < n) p[i] = load_part(parts + i * 32 + lane_id());
     m = fmaxf(m, p[i].m);
   }
   RowSum r{0.0, warp_max(m), INT32_MAX};
@@ -154,22 +159,18 @@ __device__ __forceinline__ Verdict verdict(const RowSum& row, float l, double u,
 template <class T, bool kSampled>
 __device__ __forceinline__ void block_spans(const VerifyArgs& a, int b, int j,
                                             int c, bool greedy, float scale,
-                                            uint32_t* s_top, Part* s_part) {
+                                            uint32_t* s_top) {
   const RowVecs<T> rv(row_ptr<T>(a.rows, b, j), a.rows.vocab);
   const int spans = a.split * kSWarps * a.warp_spans;
   Part* out = a.parts +
               (static_cast<int64_t>(b) * a.rows.positions + j) * spans;
   const int per = (rv.nv + spans - 1) / spans;
   for (int i = 0; i < a.warp_spans; ++i) {
-    const int at = warp_id() * a.warp_spans + i;  // in the block
-    const int w = c * kSWarps * a.warp_spans + at;
+    const int w = (c * kSWarps + warp_id()) * a.warp_spans + i;
     const Span sp = nth_span(rv.nv, w, per);
     const Part p = greedy ? warp_stats<T, true, false>(rv, sp, scale, s_top)
                           : warp_stats<T, false, true>(rv, sp, scale, s_top);
-    if (lane_id() == 0) {
-      out[w] = p;
-      s_part[at] = p;
-    }
+    if (lane_id() == 0) out[w] = p;
   }
 }
 
@@ -180,7 +181,6 @@ __device__ __forceinline__ void block_spans(const VerifyArgs& a, int b, int j,
 template <class T, bool kSampled>
 __global__ void __launch_bounds__(kSThreads, kSBlocks)
     spans_kernel(VerifyArgs a) {
-  __shared__ Part s_part[kMaxSpans];
   __shared__ uint32_t s_top;
   __shared__ int32_t s_skip;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -203,21 +203,19 @@ __global__ void __launch_bounds__(kSThreads, kSBlocks)
   if (kSampled) set = setting_of(a.set, b);
   const bool greedy = !kSampled || !(set.t > 0.0f);
   const float scale = greedy ? 0.0f : scale_of(set.t);
-  block_spans<T, kSampled>(a, b, j, c, greedy, scale, &s_top, s_part);
+  block_spans<T, kSampled>(a, b, j, c, greedy, scale, &s_top);
   if (a.rejected == nullptr || j >= k) return;
-  if (a.split > 1 && lane_id() == 0) __threadfence();
+  if (lane_id() == 0) __threadfence();  // the warp's Parts, before the count
   __syncthreads();
   if (warp_id() != 0) return;
   const int64_t at = static_cast<int64_t>(b) * (k + 1) + j;
+  int last = 0;
+  if (lane_id() == 0) last = atomicAdd(a.arrived + at, 1) == a.split - 1;
+  if (!__shfl_sync(SG_FULL_MASK, last, 0)) return;
+  __threadfence();
+  __syncwarp();
   const int spans = a.split * kSWarps * a.warp_spans;
-  const Part* row_parts = s_part;
-  if (a.split > 1) {
-    int last = 0;
-    if (lane_id() == 0) last = atomicAdd(a.arrived + at, 1) == a.split - 1;
-    if (!__shfl_sync(SG_FULL_MASK, last, 0)) return;
-    __threadfence();
-    row_parts = a.parts + at * spans;
-  }
+  const Part* row_parts = a.parts + at * spans;
   const RowSum r = greedy ? join_parts<true, false>(row_parts, spans, scale)
                         : join_parts<false, true>(row_parts, spans, scale);
   if (lane_id() != 0) return;
