@@ -100,18 +100,14 @@ __device__ __forceinline__ Part warp_stats(const RowVecs<T>& rv, Span sp,
   return Part{s, st.m, st.arg};
 }
 
-// Past the L1 cache: other blocks of the same launch may have written it.
-__device__ __forceinline__ Part load_part(const Part* p) {
-  return Part{__ldcg(&p->s), __ldcg(&p->m), __ldcg(&p->arg)};
-}
-
-// A row from the Parts of its `n` spans, in every lane of the warp.
+// A row from the Parts of its `n` spans, in every lane of the warp. kFresh:
+// past the L1 cache, since other blocks of the same launch wrote them.
 struct RowSum {
   double s;
   float m;
   int32_t arg;
 };
-template <bool kArg, bool kSum>
+template <bool kArg, bool kSum, bool kFresh = false>
 __device__ __forceinline__ RowSum join_parts(const Part* parts, int n,
                                              float scale) {
   constexpr int kPer = kMaxSpans / 32;
@@ -120,7 +116,10 @@ __device__ __forceinline__ RowSum join_parts(const Part* parts, int n,
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     p[i] = Part{0.0f, -CUDART_INF_F, INT32_MAX};
-    if (i * 32 + lane_id() < n) p[i] = load_part(parts + i * 32 + lane_id());
+    if (i * 32 + lane_id() < n) {
+      const Part* q = parts + i * 32 + lane_id();
+      p[i] = kFresh ? Part{__ldcg(&q->s), __ldcg(&q->m), __ldcg(&q->arg)} : *q;
+    }
     m = fmaxf(m, p[i].m);
   }
   RowSum r{0.0, warp_max(m), INT32_MAX};
@@ -165,6 +164,7 @@ __device__ __forceinline__ void block_spans(const VerifyArgs& a, int b, int j,
   Part* out = a.parts +
               (static_cast<int64_t>(b) * a.rows.positions + j) * spans;
   const int per = (rv.nv + spans - 1) / spans;
+#pragma unroll 1
   for (int i = 0; i < a.warp_spans; ++i) {
     const int w = (c * kSWarps + warp_id()) * a.warp_spans + i;
     const Span sp = nth_span(rv.nv, w, per);
@@ -174,12 +174,21 @@ __device__ __forceinline__ void block_spans(const VerifyArgs& a, int b, int j,
   }
 }
 
+// Greedy rows take 64 registers a thread, four blocks on an SM: those of 16
+// bits by themselves, of 32 bits when told to (37 packed requests of up to 8
+// rows of 50021: 15.3 us against 17.3; told the same, 16-bit rows spill and
+// lose 5%).
+template <class T, bool kSampled>
+constexpr int blocks_on_sm() {
+  return !kSampled && sizeof(T) == 4 ? kSBlocks + 1 : kSBlocks;
+}
+
 // a.split blocks a row, the rows of low positions first. With many rows
 // (a.rejected), the last block of a row to arrive tells whether its draft is
 // surely rejected, and rows behind such a position are left out. What is
 // left out depends on timing; the rows that the decision reads do not.
 template <class T, bool kSampled>
-__global__ void __launch_bounds__(kSThreads, kSBlocks)
+__global__ void __launch_bounds__(kSThreads, blocks_on_sm<T, kSampled>())
     spans_kernel(VerifyArgs a) {
   __shared__ uint32_t s_top;
   __shared__ int32_t s_skip;
@@ -216,8 +225,9 @@ __global__ void __launch_bounds__(kSThreads, kSBlocks)
   __syncwarp();
   const int spans = a.split * kSWarps * a.warp_spans;
   const Part* row_parts = a.parts + at * spans;
-  const RowSum r = greedy ? join_parts<true, false>(row_parts, spans, scale)
-                        : join_parts<false, true>(row_parts, spans, scale);
+  const RowSum r =
+      greedy ? join_parts<true, false, true>(row_parts, spans, scale)
+             : join_parts<false, true, true>(row_parts, spans, scale);
   if (lane_id() != 0) return;
   const int32_t x = a.draft[static_cast<int64_t>(b) * k + j];
   bool reject = x < 0 || x >= a.rows.vocab || !(r.m > -CUDART_INF_F);
