@@ -22,7 +22,7 @@ constexpr float kPlaces = 64.0f;  // places told apart in a bin
 constexpr int kWindows = 4;      // looked at before bisect_row
 constexpr int kList = 1024;      // candidates the first block can hold
 constexpr int kOwn = kList / kFThreads;
-constexpr double kFix = 17592186044416.0;  // 2^44: unit of candidates' sums
+constexpr int kFixBits = 46;     // of a candidate's weight in fixed point
 
 // What a cluster finds for a row.
 struct Kept {
@@ -424,14 +424,18 @@ __device__ __forceinline__ void plan_window(
 // One pass counts the values in bins from the largest down, a window of bins
 // at a time (mostly one is enough); the first block finds the bin of the
 // k-th value from the counts, and from counts and mean places in the bins
-// (off by about 1e-5) the bin top-p's border should lie in. A second pass sums the weights
-// ahead of those bins in 64 bits and lists the values inside them, from
-// which the first block takes both borders exactly: top-k by counting,
-// top-p by 64-bit sums, whose order does not matter (fixed point). Whether
-// the border lies in the bins looked at shows in the exact sums; if not, or
-// if the list is too short, bisect_row finds it. Without top-k, top-p's
-// share is taken of the row's fp32 sum where the border is clear of that
-// sum's error, else of its exact sum.
+// (off by about 1e-5) the bin top-p's border should lie in. A second pass
+// sums the weights ahead of those bins in 64 bits and lists the values inside
+// them, from which the first block takes both borders: top-k by counting,
+// top-p by 64-bit sums, whose order does not matter (fixed point). Their unit
+// follows the bins: 2^-46 of the weight the first of them begins with, so
+// that a sum over the whole list is off by about 2^-36 of one candidate's
+// weight, however deep it lies (with a unit for all rows, 2^-44 of the
+// largest weight, borders of top-p next to 1 missed by a token). Whether the
+// border lies in the bins looked at shows in the sums; if not, or if the list
+// is too short, bisect_row finds it. Without top-k, top-p's share is taken of
+// the row's fp32 sum where the border is clear of that sum's error, else of
+// its 64-bit sum.
 template <class T>
 __device__ void filter_row(const cooperative_groups::cluster_group& cl,
                            Share<T>& sh, int32_t k, float p, double row_sum,
@@ -520,6 +524,14 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
       int turn = 0;
       float low = -CUDART_INF_F;
       if (done) {
+        // 2^kFixBits over a power of two that no candidate's weight exceeds:
+        // values of bin b lie more than b - 1 bins below the largest
+        const int top = min(p0, k > 0 ? bk : INT32_MAX);
+        const int down = static_cast<int>(
+            fminf(static_cast<float>(max(top - 1, 0)) *
+                      (sh.scale / sh.bin_scale), 512.0f));
+        const double fix = __hiloint2double((1023 + kFixBits + down) << 20, 0);
+        const double unit = __hiloint2double((1023 - kFixBits - down) << 20, 0);
         // this thread's candidates: their keys, bins and fixed-point weights
         uint32_t key[kOwn];
         uint64_t w[kOwn];
@@ -539,7 +551,7 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
             in_k[i] = b == bk;
             in_p[i] = b >= p0 && b <= p1;
             w[i] = static_cast<uint64_t>(
-                __double2ll_rn(sh.weight(x) * kFix));
+                __double2ll_rn(sh.weight(x) * fix));
           }
         }
         // The greatest key of a set that `enough` accepts (its smallest, if
@@ -579,7 +591,7 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
             f += in_k[i] && key[i] >= tk ? w[i] : 0;
             in_p[i] = in_p[i] && key[i] >= tk;
           }
-          kept += static_cast<double>(turn_sum_u64(f, turn, fs.redl)) / kFix;
+          kept += static_cast<double>(turn_sum_u64(f, turn, fs.redl)) * unit;
           low = key_value(tk);
         }
         if (with_p) {
@@ -590,7 +602,8 @@ __device__ void filter_row(const cooperative_groups::cluster_group& cl,
 #pragma unroll
             for (int i = 0; i < kOwn; ++i)
               f += in_p[i] && key[i] >= from ? w[i] : 0;
-            return a + static_cast<double>(turn_sum_u64(f, turn, fs.redl)) / kFix;
+            return a +
+                   static_cast<double>(turn_sum_u64(f, turn, fs.redl)) * unit;
           };
           if (!(a < need - slack && mass(0) >= need + slack)) {
             done = exact ? 0 : 2;

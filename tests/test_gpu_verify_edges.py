@@ -1,0 +1,76 @@
+"""Edges of the draft-verification operators: borders deep in a row's tail,
+infinite and very large temperatures, tiny uniforms, indices beyond 32
+bits."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import verify_oracle as vo
+from suffixgpu_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+
+
+def _f64(t: torch.Tensor) -> np.ndarray:
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+def _check(got, want):
+    np.testing.assert_array_equal(got[0].cpu().numpy(), want[0])
+    np.testing.assert_array_equal(got[1].cpu().numpy(), want[1])
+
+
+def _tuned_row(g, v, t, p, top_k, miss):
+    """A row of one likely token and a tail around the border of top-p = p
+    (about 200 values in 1/16 octave), with one token's weight chosen such
+    that the mass ahead of the border's token misses p of the whole by
+    `miss` (or passes it, if negative). Returns the row and how many of its
+    tokens are kept, from sums of 80-bit floats."""
+    c = 1 - float(p)
+    depth = -np.log(c / 4600.0)
+    x = t * -(depth - 2 + 7 * torch.rand(v, generator=g))
+    x[77], x[78] = 0.0, t * np.log(2e-6)
+    tt = np.longdouble(np.float32(t))
+
+    def border(x):
+        s = np.sort(x.numpy())[::-1].astype(np.longdouble)
+        s = s[:top_k] if top_k else s
+        cum = np.cumsum(np.exp(s / tt))
+        return cum, np.longdouble(p) * cum[-1]
+    cum, need = border(x)
+    m = int((cum < need).sum())  # cum[m - 1] < need <= cum[m]
+    more = float(need - cum[m - 1] - miss) / c
+    x[78] = t * np.log(2e-6 + more)
+    cum, need = border(x)
+    assert cum[m - 2] < need < cum[m]
+    gap = float(need - cum[m - 1])
+    assert miss / 2 < gap < 2 * miss or 2 * miss < gap < miss / 2
+    return x, m + (gap > 0)
+
+
+@pytest.mark.parametrize("top_k", [0, 15_000])
+def test_top_p_borders_deep_in_the_tail(top_k):
+    """top-p 4e-6 below 1 where the border's tokens weigh 2^-30 of the
+    largest, and the mass ahead of one of them is 2e-13 more or less than
+    top-p's share.
+
+    64-bit sums of the row tell those apart: they are off by at most 2^-46
+    (1.4e-14) of it, 40 * 2^-53 for the weights (their exponents' rounding,
+    24 at a mean depth of 17 octaves, the series and 8 roundings) and 65 *
+    2^-53 for the additions on a weight's way; and top-p's share the same."""
+    n, v, t = 48, 32_003, 0.2
+    p = np.float32(1 - 4e-6)
+    g = torch.Generator().manual_seed(9 + top_k)
+    rows, want = zip(*[_tuned_row(g, v, t, p, top_k,
+                                  2e-13 if i % 2 else -2e-13)
+                       for i in range(n)])
+    logits = torch.stack(rows).to(DEV)
+    out = ops.target_probs(logits, t, top_k or None, float(p))
+    low = torch.where(out > 0, logits, float("inf")).amin(1)
+    assert ((logits >= low[:, None]) == (out > 0)).all()
+    assert (out > 0).sum(1).tolist() == list(want)
