@@ -379,6 +379,8 @@ sg_rows rows_of(const at::Tensor& t, const char* what, int64_t b,
     TORCH_CHECK_VALUE(row_start->dim() == 1 && row_start->size(0) == b,
                       "row_start must be a [B] tensor");
     r.n_rows = t.size(0);
+    TORCH_CHECK_VALUE(r.n_rows <= INT32_MAX, name +
+                      " must have fewer than 2^31 packed rows");
   } else {
     TORCH_CHECK_VALUE(t.dim() == 3, name +
                       " must be [B, K + 1, V], or [N, V] with row_start");
@@ -399,7 +401,9 @@ sg_rows rows_of(const at::Tensor& t, const char* what, int64_t b,
   return r;
 }
 
-// An index tensor as contiguous int32 on `dev`.
+// An index tensor as contiguous int32 on `dev`. 64-bit values beyond 32 bits
+// become the nearest ones, which mean the same: outside the vocabulary or the
+// packed rows, all drafts or an inactive request, no limit.
 at::Tensor index_i32(const at::Tensor& t, const char* what,
                      const at::Device& dev) {
   const at::ScalarType s = t.scalar_type();
@@ -407,7 +411,10 @@ at::Tensor index_i32(const at::Tensor& t, const char* what,
                     std::string(what) + " must be an integer tensor");
   TORCH_CHECK_VALUE(t.device() == dev,
                     std::string(what) + " is on another device");
-  return s == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+  if (s == at::kInt && t.is_contiguous()) return t;
+  if (s == at::kLong)
+    return t.clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
+  return t.to(at::kInt).contiguous();
 }
 
 // The per-request setting tensors as the struct the kernels take; `keep`

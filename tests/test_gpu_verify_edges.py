@@ -74,3 +74,51 @@ def test_top_p_borders_deep_in_the_tail(top_k):
     low = torch.where(out > 0, logits, float("inf")).amin(1)
     assert ((logits >= low[:, None]) == (out > 0)).all()
     assert (out > 0).sum(1).tolist() == list(want)
+
+
+def test_indices_beyond_32_bits():
+    """64-bit drafts, counts, row starts and top-k beyond 32 bits keep their
+    meaning: a draft outside the vocabulary, all (or no) drafts, a row
+    outside the packed ones, no limit."""
+    b, k, v = 6, 2, 300
+    g = torch.Generator().manual_seed(2)
+    logits = torch.randn(b, k + 1, v, generator=g)
+    far = 2 ** 32
+    draft = torch.randint(0, v, (b, k), generator=g)
+    logits[:, :k].scatter_(2, draft[..., None], 9.0)
+    u = torch.rand(b, k + 1, generator=g) * 0.5
+    x64, un = logits.double().numpy(), u.numpy()
+    x, u = logits.to(DEV), u.to(DEV)
+    foreign = draft.clone()
+    foreign[0, 0] += far
+    foreign[1, 1] += 2 * far
+    foreign[2, 0] -= far
+    foreign[3, 1] = 2 ** 63 - 1
+    foreign[4, 0] = -2 ** 63
+    _check(ops.verify_greedy(x, foreign.to(DEV)),
+           vo.verify_greedy(x64, foreign.numpy()))
+    _check(ops.verify_sampled(x, foreign.to(DEV), u),
+           vo.verify_sampled(x64, foreign.numpy(), un))
+    p = torch.softmax(x, 2)
+    _check(ops.verify_probs(p, foreign.to(DEV), u),
+           vo.verify_probs(_f64(p), foreign.numpy(), un))
+    nv = torch.tensor([far, -far, 1 - far, far + 1, 2 ** 63 - 1, -2 ** 63])
+    _check(ops.verify_greedy(x, draft.to(DEV), nv.to(DEV)),
+           vo.verify_greedy(x64, draft.numpy(), nv.numpy()))
+    packed = x.reshape(-1, v)
+    start = torch.tensor([0, far, 3 - far, far + 3, 2 ** 63 - 1, -2 ** 63])
+    want = vo.verify_sampled(x64.reshape(-1, v), draft.numpy(), un,
+                             row_start=start.numpy())
+    assert want[1].tolist()[1:] == [0] * 5
+    _check(ops.verify_sampled(packed, draft.to(DEV), u,
+                              row_start=start.to(DEV)), want)
+    kk = torch.tensor([far + 1, far, 2 ** 63 - 1, -2 ** 63, 1 - far, 2])
+    _check(ops.verify_sampled(x, draft.to(DEV), u, None, 3.0, kk.to(DEV)),
+           vo.verify_sampled(x64, draft.numpy(), un, None, 3.0,
+                             kk.numpy()))
+    out = ops.target_probs(x, 3.0, kk.to(DEV))
+    assert (out > 0).sum(2).tolist() == [[v] * 3] * 5 + [[2] * 3]
+    # strided, as the 32-bit ones may be
+    wide = torch.stack([foreign, draft], 2).to(DEV)[:, :, 0]
+    _check(ops.verify_greedy(x, wide),
+           vo.verify_greedy(x64, foreign.numpy()))

@@ -214,3 +214,17 @@ def test_drafter_verify_refuses_settings_without_uniforms():
         d.verify(logits, draft, temperature=0.7)
     with pytest.raises(ValueError, match="CUDA tensors"):
         d.verify(logits, draft)
+
+
+def test_refused_packed_rows_beyond_32_bit_starts():
+    """Row starts are 32-bit numbers; more packed rows than those reach are
+    refused, not cut."""
+    draft = torch.zeros(2, 1, dtype=torch.int32)
+    start = torch.zeros(2, dtype=torch.int64)
+    rows = torch.zeros(1, 4).expand(2 ** 31, 4)
+    with pytest.raises(ValueError, match="2\\^31 packed rows"):
+        ops.verify_greedy(rows, draft, row_start=start)
+    with pytest.raises(ValueError, match="2\\^31 packed rows"):
+        ops.verify_probs(rows, draft, torch.rand(2, 2), row_start=start)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        ops.verify_greedy(rows[1:], draft, row_start=start)
