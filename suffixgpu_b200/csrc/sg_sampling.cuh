@@ -372,10 +372,11 @@ __device__ __forceinline__ float scale_of(float t) {
 
 // exp((l - m) / T) in fp32. Relative error: half a step each for l - m, the
 // product and the scale act on the exponent, 3 * 2^-24 * ln2 * |z|, z = the
-// exponent of 2; plus 2^-22 of ex2.
+// exponent of 2; plus 2^-22 of ex2. Next to m = +inf nothing else has weight,
+// at an infinite temperature (scale 0) either.
 __device__ __forceinline__ float weight32(float l, float m, float scale) {
   if (l == m) return 1.0f;
-  if (!(l > -CUDART_INF_F)) return 0.0f;
+  if (!(l > -CUDART_INF_F) || m == CUDART_INF_F) return 0.0f;
   return exp2_fast((l - m) * scale);
 }
 
@@ -518,7 +519,7 @@ __device__ __forceinline__ SpanSum join_sums(const SpanSum* parts, int n,
   const float m = warp_max(p.m);
   p.arg = __reduce_min_sync(SG_FULL_MASK, p.m == m ? p.arg : INT32_MAX);
   double s = 0.0;
-  if (p.s != 0.0 && t > 0.0f)
+  if (p.s != 0.0 && t > 0.0f && (p.m == m || m < CUDART_INF_F))
     s = p.m == m ? p.s
                  : p.s * exp((static_cast<double>(p.m) -
                               static_cast<double>(m)) /

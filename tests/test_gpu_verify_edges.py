@@ -122,3 +122,47 @@ def test_indices_beyond_32_bits():
     wide = torch.stack([foreign, draft], 2).to(DEV)[:, :, 0]
     _check(ops.verify_greedy(x, wide),
            vo.verify_greedy(x64, foreign.numpy()))
+
+
+def _special_rows(v, dtype):
+    """Rows with infinite, NaN and masked entries, and one of plain ones."""
+    g = torch.Generator().manual_seed(v)
+    x = torch.randn(7, v, generator=g)
+    x[0, v // 2:] = float("inf")
+    x[1, v - 1] = float("inf")
+    x[2, ::2] = float("inf")
+    x[2, 1::2] = float("-inf")
+    x[3, ::3] = float("nan")
+    x[3, 0] = float("inf")
+    x[4, :] = float("inf")
+    x[5, 1:] = float("-inf")
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+@pytest.mark.parametrize("v", [2, 9, 1031, 40000])
+def test_infinite_temperature_and_logits(v, dtype):
+    """T = +inf on rows with +inf entries: those share the mass, with
+    and without filters, in every form. A probability is off by ex2's 2^-22
+    at most, or by the roundings of 1 / Z and of the product."""
+    x = _special_rows(v, dtype)
+    logits = x[:, None].repeat(1, 2, 1).to(DEV)
+    b, inf = x.shape[0], float("inf")
+    off = torch.zeros(b, dtype=torch.int32, device=DEV)
+    for kk, pp in ((0, 1.0), (off, 1.0), (v // 2, 1.0), (0, 0.75),
+                   (v // 2, 0.5)):
+        out = ops.target_probs(logits, inf, kk, pp).cpu().numpy()
+        k = 0 if torch.is_tensor(kk) else kk
+        for i in range(b):
+            want = vo.row_probs(_f64(x[i]), inf, k, pp)
+            for j in range(2):
+                np.testing.assert_allclose(out[i, j], want, rtol=2.0 ** -22 + 2.0 ** -23,
+                                           atol=0)
+    draft = torch.tensor([[v // 2]] * b, dtype=torch.int32)
+    u = torch.rand(b, 2, generator=torch.Generator().manual_seed(1))
+    for kk, pp in ((0, 1.0), (3, 0.6)):
+        _check(ops.verify_sampled(logits, draft.to(DEV), u.to(DEV), None, inf,
+                                  kk, pp),
+               vo.verify_sampled(_f64(logits), draft.numpy(), u.numpy(),
+                                 None, inf, kk, np.float32(pp)))
