@@ -373,25 +373,33 @@ __device__ __forceinline__ float scale_of(float t) {
 // exp((l - m) / T) in fp32. Relative error: half a step each for l - m, the
 // product and the scale act on the exponent, 3 * 2^-24 * ln2 * |z|, z = the
 // exponent of 2; plus 2^-22 of ex2. Next to m = +inf nothing else has weight,
-// at an infinite temperature (scale 0) either.
+// at an infinite temperature (scale 0) either. Where l - m passes fp32's
+// range, halves of both do not (and twice the scale is finite).
 __device__ __forceinline__ float weight32(float l, float m, float scale) {
   if (l == m) return 1.0f;
   if (!(l > -CUDART_INF_F) || m == CUDART_INF_F) return 0.0f;
-  return exp2_fast((l - m) * scale);
+  const float d = l - m;
+  return exp2_fast(d > -CUDART_INF_F ? d * scale
+                                     : (0.5f * l - 0.5f * m) * (2.0f * scale));
 }
+
+// Scales below this one (temperatures above 2^100) leave weight where l - m
+// passes fp32's range, and have no second part: they are left to weight32.
+constexpr float kFlatScale = 1.138e-30f;
 
 // The scale in two parts, so that its rounding, which would act on all
 // weights alike and shift a row's probabilities by 2^-24 times their mean
 // depth, does not count: z = d * (hi + lo) is rounded once, by itself. hi is
-// rounded down and lo above 0, so that -inf keeps its sign.
+// rounded down and lo above 0 (by the smallest number there is, next to
+// nothing beside any scale above kFlatScale), so that -inf keeps its sign.
 struct FineScale {
   float hi, lo;
 };
 __device__ __forceinline__ FineScale fine_scale_of(float t) {
   FineScale f;
   const double s = 1.4426950408889634074 / static_cast<double>(t);
-  f.hi = __double2float_rd(s);
-  f.lo = fmaxf(static_cast<float>(s - static_cast<double>(f.hi)), 1e-30f);
+  f.hi = s < kFlatScale ? static_cast<float>(s) : __double2float_rd(s);
+  f.lo = fmaxf(static_cast<float>(s - static_cast<double>(f.hi)), 1.4e-45f);
   return f;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -484,9 +492,9 @@ __device__ __forceinline__ void take_vecs(const uint4 (&raw)[U], Index index,
       acc = add2(acc, p[0]);
     }
     float ts = acc.x + acc.y;
-    // NaN: masked NaN logits, +inf, or an infinite temperature's scale of 0
-    // on -inf; such vectors are summed again with each case told apart
-    if (ts != ts) {
+    // NaN: masked NaN logits, or +inf; such vectors, and all at the largest
+    // temperatures, are summed again with each case told apart
+    if (ts != ts || scale < kFlatScale) {
       ts = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {

@@ -813,7 +813,7 @@ __device__ __forceinline__ void write_kept(const Share<T>& sh, float* orow,
                                            float t) {
   const float inv_z = static_cast<float>(1.0 / z);
   const FineScale f = fine_scale_of(t);
-  if (m == CUDART_INF_F || t == CUDART_INF_F) {
+  if (m == CUDART_INF_F || f.hi < kFlatScale) {
     write_share(sh, orow, [&](float2 x) {
       return make_float2(x.x >= low ? weight32(x.x, m, f.hi) * inv_z : 0.0f,
                          x.y >= low ? weight32(x.y, m, f.hi) * inv_z : 0.0f);

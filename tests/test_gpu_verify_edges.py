@@ -166,3 +166,49 @@ def test_infinite_temperature_and_logits(v, dtype):
                                   kk, pp),
                vo.verify_sampled(_f64(logits), draft.numpy(), u.numpy(),
                                  None, inf, kk, np.float32(pp)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [5, 1009, 20011])
+@pytest.mark.parametrize("t", [1e20, 1e24, 1e29, 2e30, 1e37, 3e38,
+                               float("inf")])
+def test_very_large_temperatures(t, v, dtype):
+    """Temperatures up to fp32's largest number and +inf, on logits as large:
+    spread out like the temperature, and near both ends of the type's range,
+    where l - m passes fp32's.
+
+    A probability's error in half steps (2^-24): 5 for each unit of depth
+    (l - m) / T (l - m and the product one each, the scale 2.8 where it is
+    below the smallest normal number), 4 for ex2, 2 for 1 / Z and the
+    product, 20 additions, 2 for the scale's other rounding in the sum."""
+    g = torch.Generator().manual_seed(v)
+    big = torch.finfo(dtype).max
+    size = min(t, big / 8)
+    x = torch.randn(4, v, generator=g)
+    x = (x * size).clamp(-big, big)
+    ends = torch.rand(v, generator=g)
+    x[1] = torch.where(ends < 0.3, big, torch.where(ends < 0.6, -big, 0.0))
+    x[2] = torch.where(ends < 0.5, -big, x[2])
+    x[2, 0] = big
+    x[3] = torch.where(ends < 0.5, float("-inf"), x[3])
+    x = x.to(dtype)
+    x = torch.where(torch.isinf(x) & (x > 0), big, x)
+    logits = x[:, None].repeat(1, 2, 1).to(DEV)
+    x64 = _f64(x)
+    tt = float(np.float32(t))
+    for k, p in ((0, 1.0), (v // 2, 0.7)):
+        out = _f64(ops.target_probs(logits, t, k, p))
+        for i in range(4):
+            want = vo.row_probs(x64[i], tt, k, float(np.float32(p)))
+            m = x64[i].max()
+            depth = np.where(want > 0, m - x64[i], 0.0) / tt
+            tol = 2.0 ** -24 * (5 * depth + 28) * want
+            assert (np.abs(out[i] - want) <= tol + 2.0 ** -126).all()
+            assert (out[i][:, want == 0] == 0).all()
+    draft = torch.randint(0, v, (4, 1), generator=g)
+    u = torch.rand(4, 2, generator=g)
+    for k, p in ((0, 1.0), (v // 2, 0.7)):
+        _check(ops.verify_sampled(logits, draft.to(DEV), u.to(DEV), None, t,
+                                  k, p),
+               vo.verify_sampled(_f64(logits), draft.numpy(), u.numpy(),
+                                 None, np.float32(t), k, np.float32(p)))
