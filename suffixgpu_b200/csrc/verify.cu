@@ -143,14 +143,15 @@ static int warp_spans_of(int64_t vocab, int elems, int split) {
       std::min<int64_t>(want, kMaxSpans / (split * kSWarps)));
 }
 
-// Whether a draft is accepted, where fp32 weights can tell.
+// Whether a draft is accepted, where fp32 weights can tell: not within their
+// errors, nor where both sides are as small as a weight that is flushed to 0.
 enum Verdict : int { kReject = 0, kAccept = 1, kUnsure = 2 };
 
 __device__ __forceinline__ Verdict verdict(const RowSum& row, float l, double u,
                                            float scale, double guard) {
   const double w = weight32(l, row.m, scale);
   const double uz = u * row.s;
-  if (!(fabs(uz - w) > guard * uz + kDeepGuard * w)) return kUnsure;
+  if (!(fabs(uz - w) > guard * uz + kDeepGuard * w + 1.2e-38)) return kUnsure;
   return uz < w ? kAccept : kReject;
 }
 

@@ -212,3 +212,30 @@ def test_very_large_temperatures(t, v, dtype):
                                   k, p),
                vo.verify_sampled(_f64(logits), draft.numpy(), u.numpy(),
                                  None, np.float32(t), k, np.float32(p)))
+
+
+@pytest.mark.parametrize("b", [1, 160])
+@pytest.mark.parametrize("v", [3, 2049])
+def test_tiny_uniforms_and_probabilities(v, b):
+    """Uniforms and drafted tokens' probabilities below the smallest normal
+    fp32 number, next to one another: u < P(x) as 64 bits have it. Few
+    requests and (b x 4 rows) more than one launch decides."""
+    deep = torch.tensor([-86.5, -87.0, -87.5, -88.5, -90.0, -95.0, -102.0])
+    g = torch.Generator().manual_seed(b + v)
+    x = torch.full((b, 4, v), float("-inf"))
+    x[..., 1] = 0.0
+    d = deep[torch.randint(0, 7, (b, 3), generator=g)]
+    d[:, 0] = -90.0
+    x[:, :3, 0] = d
+    u = torch.exp(d.double()) * torch.tensor([0.25, 0.5, 0.9, 1.1, 2.0])[
+        torch.randint(0, 5, (b, 3), generator=g)]
+    u = torch.cat([u.float(), torch.rand(b, 1, generator=g)], 1)
+    u[:, 0] = 5e-40
+    draft = torch.zeros(b, 3, dtype=torch.int32)
+    want = vo.verify_sampled(x.double().numpy(), draft.numpy(), u.numpy())
+    assert (want[1] > 1).all()
+    _check(ops.verify_sampled(x.to(DEV), draft.to(DEV), u.to(DEV)), want)
+    _check(ops.verify_sampled(x.to(DEV), draft.to(DEV), u.to(DEV), None, 1.0,
+                              0, 1 - 2.0 ** -24),
+           vo.verify_sampled(x.double().numpy(), draft.numpy(), u.numpy(),
+                             None, 1.0, 0, np.float32(1 - 2.0 ** -24)))
