@@ -45,30 +45,30 @@ int num_sms();
 int current_device();
 
 // Make `kernel` launchable with `bytes` of dynamic shared memory on the
-// current device. `cache` (one slot per device) remembers what was set.
-// Static + dynamic shared memory must fit the per-block opt-in limit.
+// current device: its limit is raised once, to the largest one (static +
+// dynamic shared memory must fit the per-block opt-in limit), so that calls
+// of different sizes from several threads all set the same. `cache` (one slot
+// per device) holds that limit once it is set.
 template <class Kernel>
 inline int ensure_dyn_smem(Kernel* kernel, size_t bytes, int* cache) {
   if (bytes <= 48 * 1024) return SG_OK;
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return SG_ERR_CUDA;
-  if (static_cast<int>(bytes) <= cache[dev]) return SG_OK;
-  cudaFuncAttributes fa;
-  cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return SG_ERR_CUDA;
+  int limit = __atomic_load_n(cache + dev, __ATOMIC_ACQUIRE);
+  if (limit == 0) {
+    cudaFuncAttributes fa{};
+    cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+    limit = max_dyn_smem() - static_cast<int>(fa.sharedSizeBytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(
+          kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      return SG_ERR_CUDA;
+    }
+    __atomic_store_n(cache + dev, limit, __ATOMIC_RELEASE);
   }
-  if (bytes + fa.sharedSizeBytes > static_cast<size_t>(max_dyn_smem()))
-    return SG_ERR_UNSUPPORTED;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(bytes));
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return SG_ERR_CUDA;
-  }
-  cache[dev] = static_cast<int>(bytes);
-  return SG_OK;
+  return bytes <= static_cast<size_t>(limit) ? SG_OK : SG_ERR_UNSUPPORTED;
 }
 
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) {
