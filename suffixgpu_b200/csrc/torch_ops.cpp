@@ -18,6 +18,8 @@
 // target_probs wrap the draft-verification entry points; their argument
 // checks run before any CUDA call (and raise ValueError).
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -612,9 +614,6 @@ at::Tensor target_probs(const at::Tensor& logits,
                         double top_p_all) {
   TORCH_CHECK_VALUE(logits.dim() == 2 || logits.dim() == 3,
                     "logits must be [N, V] or [B, J, V]");
-  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && logits.requires_grad()),
-                    "target_probs has no backward pass: detach the logits "
-                    "or call it under torch.no_grad()");
   const at::Tensor rows = logits.dim() == 3 ? logits : logits.unsqueeze(1);
   sg_rows r = rows_of(rows, "logits", rows.size(0), rows.size(1),
                       c10::nullopt);
@@ -630,6 +629,34 @@ at::Tensor target_probs(const at::Tensor& logits,
                sg_target_probs(&r, &s, out.data_ptr<float>(),
                                stream_for(rows)));
   return out;
+}
+
+// In front of target_probs wherever derivatives are recorded (backward,
+// forward mode, function transforms): it has none.
+at::Tensor target_probs_autograd(const at::Tensor& logits,
+                                 const c10::optional<at::Tensor>& temperature,
+                                 const c10::optional<at::Tensor>& top_k,
+                                 const c10::optional<at::Tensor>& top_p,
+                                 double temperature_all, int64_t top_k_all,
+                                 double top_p_all) {
+  const bool backward = at::GradMode::is_enabled();
+  auto check = [&](const at::Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(
+        !(backward && t.requires_grad()) && !t._fw_grad(0).defined(),
+        std::string("target_probs has no backward pass and no forward-mode "
+                    "derivative: detach the ") + what +
+            " (for the former, torch.no_grad() does as well)");
+  };
+  check(logits, "logits");
+  if (temperature.has_value()) check(*temperature, "temperature");
+  if (top_p.has_value()) check(*top_p, "top_p");
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("suffixgpu_b200::target_probs", "")
+          .typed<decltype(target_probs)>();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, temperature, top_k, top_p, temperature_all,
+                 top_k_all, top_p_all);
 }
 
 }  // namespace
@@ -682,6 +709,10 @@ TORCH_LIBRARY_IMPL(suffixgpu_b200, CompositeExplicitAutograd, m) {
   m.impl("verify_sampled", &verify_sampled);
   m.impl("verify_probs", &verify_probs);
   m.impl("target_probs", &target_probs);
+}
+
+TORCH_LIBRARY_IMPL(suffixgpu_b200, Autograd, m) {
+  m.impl("target_probs", &target_probs_autograd);
 }
 
 TORCH_LIBRARY_IMPL(suffixgpu_b200, CUDA, m) {

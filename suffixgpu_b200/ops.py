@@ -346,7 +346,8 @@ def target_probs(logits: torch.Tensor,
     """The target's probabilities under verify_sampled's temperature, top_k
     and top_p, float32 in the shape of logits ([N, V] with [N] settings, or
     [B, J, V] with [B] settings; float32, bfloat16 or float16). Dropped
-    tokens are exactly 0; a row of -inf gives zeros. No backward pass."""
+    tokens are exactly 0; a row of -inf gives zeros. No backward pass and no
+    forward-mode derivative: inputs that ask for one are refused."""
     t, t_all = _setting(temperature, 1.0)
     k, k_all = _setting(top_k, 0)
     p, p_all = _setting(top_p, 1.0)

@@ -228,3 +228,33 @@ def test_refused_packed_rows_beyond_32_bit_starts():
         ops.verify_probs(rows, draft, torch.rand(2, 2), row_start=start)
     with pytest.raises(ValueError, match="CUDA tensors"):
         ops.verify_greedy(rows[1:], draft, row_start=start)
+
+
+def test_target_probs_refuses_every_kind_of_derivative():
+    """Forward mode, function transforms and settings that need a gradient,
+    none of which the operator has, are refused like a backward pass."""
+    import torch.autograd.forward_ad as fwad
+    x = torch.randn(2, 9)
+    t = torch.ones(2)
+    match = "no backward pass"
+    with fwad.dual_level():
+        with pytest.raises(ValueError, match=match):
+            ops.target_probs(fwad.make_dual(x, x))
+        with pytest.raises(ValueError, match=match):
+            ops.target_probs(x, fwad.make_dual(t, t))
+    with pytest.raises(ValueError, match=match):
+        torch.func.grad(lambda y: ops.target_probs(y).sum())(x)
+    with pytest.raises(ValueError, match=match):
+        torch.func.jvp(ops.target_probs, (x,), (x,))
+    for kw in (dict(temperature=t.clone().requires_grad_()),
+               dict(top_p=t.clone().requires_grad_())):
+        with pytest.raises(ValueError, match=match):
+            ops.target_probs(x, **kw)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            ops.target_probs(x, **kw)
+    with torch.inference_mode(), pytest.raises(ValueError, match="CUDA"):
+        ops.target_probs(x)
+    # the verified tokens are whole numbers, without a derivative
+    logits, draft, u = _args()
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.verify_sampled(logits.requires_grad_(), draft, u)
