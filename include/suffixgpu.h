@@ -224,7 +224,8 @@ int sg_expand_chain(const int32_t* cont, int32_t rows, int32_t max_occ,
 #define SG_BF16 1
 #define SG_F16 2
 
-/* Rows of logits or probabilities, a row for each request and position.
+/* Rows of logits or probabilities, a row for each request and position; data
+ * lies on its type's boundary (SG_ERR_INVALID otherwise).
  * row_start NULL: row j of request b starts at element
  * b * stride_b + j * stride_j. Otherwise rows are packed, stride_b elements
  * apart, and row j of request b is row row_start[b] + j of n_rows; a row
@@ -254,8 +255,9 @@ typedef struct sg_sampling {
   int32_t pad_;
 } sg_sampling;
 
-/* Workspace bytes of sg_verify_greedy and sg_verify_sampled. Calls that may overlap on the GPU (other streams, other
- * graphs) need workspaces of their own. */
+/* Workspace bytes of sg_verify_greedy and sg_verify_sampled. Calls that may
+ * overlap on the GPU (other streams, other graphs) need workspaces of their
+ * own. */
 size_t sg_verify_workspace_size(int32_t batch, int32_t positions);
 
 /* Verification at temperature 0: each accepted draft equals its row's first

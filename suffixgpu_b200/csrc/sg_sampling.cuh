@@ -194,6 +194,8 @@ inline int check_rows(const sg_rows* r, bool probs) {
   if (r->dtype < SG_F32 || r->dtype > SG_F16) return SG_ERR_INVALID;
   if (probs && r->dtype != SG_F32) return SG_ERR_UNSUPPORTED;
   if (r->batch == 0 || r->positions == 0) return SG_OK;
+  const uintptr_t size = r->dtype == SG_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(r->data) % size) return SG_ERR_INVALID;
   if (r->row_start != nullptr) {
     if (r->n_rows < 0 || r->stride_b < 0) return SG_ERR_INVALID;
     if (r->n_rows > 0 && !r->data) return SG_ERR_INVALID;

@@ -258,3 +258,34 @@ def test_target_probs_refuses_every_kind_of_derivative():
     logits, draft, u = _args()
     with pytest.raises(ValueError, match="CUDA"):
         ops.verify_sampled(logits.requires_grad_(), draft, u)
+
+
+def test_misaligned_rows_at_the_c_abi():
+    """Rows that do not start on their type's boundary are refused (a 16- or
+    32-bit load there would fault)."""
+    L = _lib.lib()
+    s = _lib.Sampling(temperature_all=1.0, top_p_all=1.0)
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        for off in range(1, size):
+            r = _lib.Rows(data=4096 + off, dtype=dtype, batch=2, positions=3,
+                          vocab=9, stride_b=27, stride_j=9)
+            p = _lib.Rows(data=4096 + off, dtype=dtype, batch=2, positions=3,
+                          vocab=9, stride_b=9, row_start=4096, n_rows=6)
+            for rows in (r, p):
+                assert L.sg_verify_greedy(ctypes.byref(rows), 4096, None,
+                                          4096, 4096, 4096, 0, None) == 1
+                assert L.sg_verify_sampled(
+                    ctypes.byref(rows), ctypes.byref(s), 4096, None, 4096,
+                    4096, 4096, 4096, 0, None) == 1
+            # without an output: 1 from the check, were it to pass as well
+            assert L.sg_target_probs(ctypes.byref(r), ctypes.byref(s), None,
+                                     None) == 1
+    good = _lib.Rows(data=4096, dtype=0, batch=2, positions=3, vocab=9,
+                     stride_b=27, stride_j=9)
+    bad = _lib.Rows(data=4097, dtype=0, batch=2, positions=2, vocab=9,
+                    stride_b=27, stride_j=9)
+    assert L.sg_verify_probs(ctypes.byref(good), ctypes.byref(bad), 4096,
+                             None, 4096, 4096, 4096, None) == 1
+    # a start on the boundary passes the check (and lacks a workspace)
+    assert L.sg_verify_greedy(ctypes.byref(good), 4096, None, 4096, 4096,
+                              4096, 0, None) == 2
