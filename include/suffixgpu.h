@@ -287,8 +287,8 @@ int sg_verify_probs(const sg_rows* probs, const sg_rows* draft_probs,
 
 /* The target's probabilities P of every row, out [B, positions, V] fp32
  * (contiguous). Here and in sg_verify_sampled with top-k or top-p, a row has
- * to fit the shared memory of 8 SMs: SG_ERR_UNSUPPORTED beyond about 1.3 MB
- * (a vocabulary of 350 thousand in fp32). */
+ * to fit the shared memory of 8 SMs: SG_ERR_UNSUPPORTED beyond about 1.5 MB
+ * (a vocabulary of 380 thousand in fp32). */
 int sg_target_probs(const sg_rows* logits, const sg_sampling* sampling,
                     float* out, sg_stream_t stream);
 

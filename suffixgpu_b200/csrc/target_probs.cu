@@ -422,7 +422,9 @@ __device__ __forceinline__ void plan_window(
 // top-p (0 < p < 1) or both; left in fs.low and fs.z of every block.
 //
 // One pass counts the values in bins from the largest down, a window of bins
-// at a time (mostly one is enough); the first block finds the bin of the
+// at a time (one or two mostly: a window is 10.7 logits at T = 1, and the
+// border at p = 0.95 to 0.99 lies 10.5 to 13 down in rows of a normal bulk
+// and a few likely tokens); the first block finds the bin of the
 // k-th value from the counts, and from counts and mean places in the bins
 // (off by about 1e-5) the bin top-p's border should lie in. A second pass
 // sums the weights ahead of those bins in 64 bits and lists the values inside
@@ -433,7 +435,8 @@ __device__ __forceinline__ void plan_window(
 // weight, however deep it lies (with a unit for all rows, 2^-44 of the
 // largest weight, borders of top-p next to 1 missed by a token). Whether the
 // border lies in the bins looked at shows in the sums; if not, or if the list
-// is too short, bisect_row finds it. Without top-k, top-p's share is taken of
+// is too short, or the border lies beyond the windows (k-th values of -inf
+// among them), bisect_row finds it. Without top-k, top-p's share is taken of
 // the row's fp32 sum where the border is clear of that sum's error, else of
 // its 64-bit sum.
 template <class T>
@@ -1041,7 +1044,7 @@ __global__ void __launch_bounds__(kFThreads, kStatBlocks)
 // blocks to fill the machine where rows are few. 32 KiB where rows are
 // written; 64 KiB for the statistics, whose passes cost every block much the
 // same whatever its share (128 x 33 rows of 128256 bf16, top-k and top-p:
-// 371 us against 504, and 566 with 128 KiB).
+// 371 us against 504, and 566 with 128 KiB; not measured with few rows).
 static int row_cluster(const sg_rows& r, int64_t share) {
   const int64_t rows = static_cast<int64_t>(r.batch) * r.positions;
   const int64_t bytes = r.vocab * (r.dtype == SG_F32 ? 4 : 2);

@@ -239,3 +239,27 @@ def test_tiny_uniforms_and_probabilities(v, b):
                               0, 1 - 2.0 ** -24),
            vo.verify_sampled(x.double().numpy(), draft.numpy(), u.numpy(),
                              None, 1.0, 0, np.float32(1 - 2.0 ** -24)))
+
+
+def test_largest_vocabulary_held_on_chip():
+    """380 thousand fp32 logits a row, with filters and without; 420 thousand
+    are refused."""
+    v = 380_000
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 1, v, generator=g) * 3
+    draft = torch.empty(2, 0, dtype=torch.int32)
+    u = torch.rand(2, 1, generator=g)
+    _check(ops.verify_sampled(x.to(DEV), draft.to(DEV), u.to(DEV), None, 0.9,
+                              40, 0.9),
+           vo.verify_sampled(x.double().numpy(), draft.numpy(), u.numpy(),
+                             None, np.float32(0.9), 40, np.float32(0.9)))
+    out = ops.target_probs(x.to(DEV), 0.9)
+    want = torch.softmax(x.double() / float(np.float32(0.9)), 2)
+    # as _probs_close in the sizes' tests, with 20 additions more: depth is
+    # at most 2 * 5.5 * 3 / 0.9 < 40
+    np.testing.assert_allclose(out.double().cpu(), want,
+                               rtol=2.0 ** -24 * (3 * 40 + 28))
+    far = torch.zeros(1, 420_000, device=DEV)
+    for k in (0, 40):
+        with pytest.raises(RuntimeError, match="beyond supported limits"):
+            ops.target_probs(far, 0.9, k)
