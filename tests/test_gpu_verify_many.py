@@ -237,3 +237,39 @@ def test_captured_decode_loop(sampled, enable_global):
         np.testing.assert_array_equal(nv.cpu().numpy(), nv_o)
     assert accepted > 0
     del graph
+
+
+def test_calls_from_several_threads():
+    """Four threads, each on a stream of its own with a vocabulary of its
+    own, whose rows need different amounts of shared memory."""
+    import threading
+
+    def forms(rows, draft, nv, u, t):
+        return [*ops.verify_greedy(rows, draft, nv),
+                *ops.verify_sampled(rows, draft, u, nv, t),
+                *ops.verify_sampled(rows, draft, u, nv, t, 30, 0.9),
+                ops.target_probs(rows, t),
+                ops.target_probs(rows, t, top_p=0.9)]
+    sets = [_case(v, 3, 2, v, torch.float32, False)[:5]
+            for v in (9001, 90_001, 250_001, 40_001)]
+    torch.cuda.synchronize()
+    gate, got, errors = threading.Barrier(4, timeout=60), [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                gate.wait()
+                for _ in range(5):
+                    got[i] = forms(*sets[i])
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # reported by the main thread
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors
+    for x, out in zip(sets, got):
+        for a, b in zip(forms(*x), out):
+            assert torch.equal(a, b)
