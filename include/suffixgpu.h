@@ -255,6 +255,14 @@ typedef struct sg_sampling {
   int32_t pad_;
 } sg_sampling;
 
+/* 64-bit drafts, counts, row starts or top-k as the 32-bit ones that the
+ * calls below take: the nearest, so that what lies beyond 32 bits keeps its
+ * meaning (a foreign token or row, all drafts, none, no limit). src is
+ * [rows, cols] with strides in elements, out contiguous. */
+int sg_clamp_i32(const int64_t* src, int64_t rows, int64_t cols,
+                 int64_t stride_row, int64_t stride_col, int32_t* out,
+                 sg_stream_t stream);
+
 /* Workspace bytes of sg_verify_greedy and sg_verify_sampled. Calls that may
  * overlap on the GPU (other streams, other graphs) need workspaces of their
  * own. */

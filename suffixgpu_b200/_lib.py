@@ -157,6 +157,8 @@ _SIGS: dict[str, list] = {
                                 c_int32, c_float, c_float, c_float, c_float,
                                 c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_void_p],
+    "sg_clamp_i32": [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                     c_void_p],
     "sg_verify_greedy": [POINTER(Rows), c_void_p, c_void_p, c_void_p,
                          c_void_p, c_void_p, c_size_t, c_void_p],
     "sg_verify_sampled": [POINTER(Rows), POINTER(Sampling), c_void_p,

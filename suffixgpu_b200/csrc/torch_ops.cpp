@@ -378,8 +378,6 @@ sg_rows rows_of(const at::Tensor& t, const char* what, int64_t b,
   if (row_start.has_value()) {
     TORCH_CHECK_VALUE(t.dim() == 2, name +
                       " must be [N, V] when row_start is given");
-    TORCH_CHECK_VALUE(row_start->dim() == 1 && row_start->size(0) == b,
-                      "row_start must be a [B] tensor");
     r.n_rows = t.size(0);
     TORCH_CHECK_VALUE(r.n_rows <= INT32_MAX, name +
                       " must have fewer than 2^31 packed rows");
@@ -403,9 +401,20 @@ sg_rows rows_of(const at::Tensor& t, const char* what, int64_t b,
   return r;
 }
 
-// An index tensor as contiguous int32 on `dev`. 64-bit values beyond 32 bits
-// become the nearest ones, which mean the same: outside the vocabulary or the
-// packed rows, all drafts or an inactive request, no limit.
+// An uninitialised tensor on the device of `like`, past the dispatcher.
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes,
+                    at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
+
+sg_stream_t stream_for(const at::Tensor& t) {
+  return reinterpret_cast<sg_stream_t>(
+      c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
+}
+
+// A [B] or [B, K] index tensor as contiguous int32 on `dev`. 64-bit values
+// beyond 32 bits become the nearest ones, which mean the same: outside the
+// vocabulary or the packed rows, all drafts or an inactive request, no limit.
 at::Tensor index_i32(const at::Tensor& t, const char* what,
                      const at::Device& dev) {
   const at::ScalarType s = t.scalar_type();
@@ -414,8 +423,17 @@ at::Tensor index_i32(const at::Tensor& t, const char* what,
   TORCH_CHECK_VALUE(t.device() == dev,
                     std::string(what) + " is on another device");
   if (s == at::kInt && t.is_contiguous()) return t;
-  if (s == at::kLong)
-    return t.clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
+  if (s == at::kLong && t.is_cuda()) {
+    const c10::cuda::CUDAGuard guard(t.device());
+    at::Tensor r = empty_on(t, t.sizes(), at::kInt);
+    const bool wide = t.dim() == 2;
+    check_status("sg_clamp_i32",
+                 sg_clamp_i32(t.data_ptr<int64_t>(), t.size(0),
+                              wide ? t.size(1) : 1, t.stride(0),
+                              wide ? t.stride(1) : 0, r.data_ptr<int32_t>(),
+                              stream_for(t)));
+    return r;
+  }
   return t.to(at::kInt).contiguous();
 }
 
@@ -455,12 +473,6 @@ sg_sampling sampling_of(const c10::optional<at::Tensor>& temperature,
   return s;
 }
 
-// An uninitialised tensor on the device of `like`, past the dispatcher.
-at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes,
-                    at::ScalarType dtype) {
-  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
-}
-
 // What the three verify operators share: the checked index tensors, the
 // output buffer and the launch stream.
 struct VerifyCall {
@@ -485,8 +497,11 @@ struct VerifyCall {
                         "num_valid must be a [B] tensor");
       num_valid = index_i32(*num_valid_in, "num_valid", dev);
     }
-    if (row_start_in.has_value())
+    if (row_start_in.has_value()) {
+      TORCH_CHECK_VALUE(row_start_in->dim() == 1 && row_start_in->size(0) == b,
+                        "row_start must be a [B] tensor");
       row_start = index_i32(*row_start_in, "row_start", dev);
+    }
     if (uniforms_in.has_value()) {
       TORCH_CHECK_VALUE(uniforms_in->scalar_type() == at::kFloat &&
                             uniforms_in->dim() == 2 &&
@@ -517,11 +532,6 @@ struct VerifyCall {
     return {std::move(ids), std::move(counts)};
   }
 };
-
-sg_stream_t stream_for(const at::Tensor& t) {
-  return reinterpret_cast<sg_stream_t>(
-      c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
-}
 
 // A workspace of the call's own: calls on other streams and other captured
 // graphs never share one.

@@ -891,6 +891,32 @@ __global__ void __launch_bounds__(kCThreads, 5) probs_kernel(ProbArgs a) {
   if (leader) emit(drow, s, tok, k, out, a.count + b);
 }
 
+// 64-bit indices as the nearest 32-bit ones, a thread each. The launch bounds
+// it: 8 x 5 x 32000 greedy with 64-bit drafts takes 12.3 us a call, 8.9 with
+// 32-bit ones (19.3 with a library's clamp and conversion).
+struct ClampArgs {
+  const int64_t* src;
+  int64_t n, cols, stride_row, stride_col;
+  int32_t* out;
+};
+constexpr int kClampThreads = 256;
+constexpr int64_t kClampBlocks = 148 * 8;
+
+__global__ void __launch_bounds__(kClampThreads) clamp_kernel(ClampArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kClampThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kClampThreads +
+                   threadIdx.x;
+       i < a.n; i += step) {
+    const int64_t x =
+        a.src[i / a.cols * a.stride_row + i % a.cols * a.stride_col];
+    a.out[i] = static_cast<int32_t>(
+        max(static_cast<int64_t>(INT32_MIN),
+            min(static_cast<int64_t>(INT32_MAX), x)));
+  }
+}
+
 static int check_workspace(const sg_rows* r, const void* ws, size_t bytes) {
   const size_t need = sg_verify_workspace_size(r->batch, r->positions);
   if (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15))
@@ -980,6 +1006,22 @@ static int verify(const sg_rows* logits, const sg_sampling* sampling,
 }  // namespace sg
 
 using namespace sg;
+
+extern "C" int sg_clamp_i32(const int64_t* src, int64_t rows, int64_t cols,
+                            int64_t stride_row, int64_t stride_col,
+                            int32_t* out, sg_stream_t stream) {
+  NvtxScope nvtx("sg_clamp_i32");
+  if (rows < 0 || cols < 0 || stride_row < 0 || stride_col < 0)
+    return SG_ERR_INVALID;
+  if (rows == 0 || cols == 0) return SG_OK;
+  if (!src || !out) return SG_ERR_INVALID;
+  if (rows > INT64_MAX / cols) return SG_ERR_UNSUPPORTED;
+  const ClampArgs a{src, rows * cols, cols, stride_row, stride_col, out};
+  const int64_t blocks = std::min(kClampBlocks, ceil_div(a.n, kClampThreads));
+  return launch_after(clamp_kernel, static_cast<unsigned>(blocks),
+                      kClampThreads, 1, a,
+                      reinterpret_cast<cudaStream_t>(stream));
+}
 
 extern "C" size_t sg_verify_workspace_size(int32_t batch, int32_t positions) {
   if (batch <= 0 || positions <= 0) return 0;

@@ -263,3 +263,30 @@ def test_largest_vocabulary_held_on_chip():
     for k in (0, 40):
         with pytest.raises(RuntimeError, match="beyond supported limits"):
             ops.target_probs(far, 0.9, k)
+
+
+@pytest.mark.parametrize("b,k", [(1, 0), (1, 1), (5, 3), (300, 2),
+                                 (70_000, 5)])
+def test_64_bit_indices_of_any_layout(b, k):
+    """Contiguous, transposed, sliced and expanded 64-bit tensors give what
+    the 32-bit ones do (70 thousand requests: more elements than threads)."""
+    v = 5
+    g = torch.Generator().manual_seed(b)
+    x = torch.randn(b, k + 1, v, generator=g).to(DEV)
+    draft = torch.randint(-1, v + 1, (b, k), generator=g).to(DEV)
+    nv = torch.randint(-1, k + 2, (b,), generator=g).to(DEV)
+    kk = torch.randint(0, v + 2, (b,), generator=g).to(DEV)
+    u = torch.rand(b, k + 1, generator=g).to(DEV)
+
+    def both(draft, nv, kk):
+        a = ops.verify_sampled(x, draft, u, nv, 0.8, kk)
+        c = ops.verify_sampled(x, draft.int().contiguous(), u,
+                               nv.int().contiguous(), 0.8,
+                               kk.int().contiguous())
+        assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+    both(draft, nv, kk)
+    both(draft.t().contiguous().t(), torch.stack([nv, kk], 1)[:, 0],
+         torch.stack([nv, kk], 1)[:, 1])
+    both(torch.cat([draft, draft], 1)[:, k:], nv[:1].expand(b),
+         kk[:1].expand(b))
+    both(draft[:1].expand(b, k), nv, kk)

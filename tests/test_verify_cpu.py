@@ -289,3 +289,21 @@ def test_misaligned_rows_at_the_c_abi():
     # a start on the boundary passes the check (and lacks a workspace)
     assert L.sg_verify_greedy(ctypes.byref(good), 4096, None, 4096, 4096,
                               4096, 0, None) == 2
+
+
+def test_refused_row_starts_and_clamps():
+    draft = torch.zeros(2, 1, dtype=torch.int64)
+    rows = torch.zeros(4, 5)
+    for start in (torch.tensor(0), torch.zeros(3, dtype=torch.int64),
+                  torch.zeros(2, 1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match=r"row_start must be a \[B\]"):
+            ops.verify_greedy(rows, draft, row_start=start)
+    L = _lib.lib()
+    one = 4096  # never dereferenced
+    assert L.sg_clamp_i32(None, 0, 3, 3, 1, None, None) == 0
+    assert L.sg_clamp_i32(None, 3, 0, 3, 1, None, None) == 0
+    assert L.sg_clamp_i32(None, 2, 3, 3, 1, one, None) == 1
+    assert L.sg_clamp_i32(one, 2, 3, 3, 1, None, None) == 1
+    for bad in ((-1, 3, 3, 1), (2, -1, 3, 1), (2, 3, -3, 1), (2, 3, 3, -1)):
+        assert L.sg_clamp_i32(one, *bad, one, None) == 1
+    assert L.sg_clamp_i32(one, 2 ** 62, 4, 4, 1, one, None) == 4
